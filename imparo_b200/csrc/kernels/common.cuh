@@ -21,6 +21,7 @@
 #define IMPARO_ST_PAGE_RANGE 2
 #define IMPARO_ST_SLOT_RANGE 3
 #define IMPARO_ST_WAIT_LIMIT 4
+#define IMPARO_ST_STEP_SIZE 5
 
 namespace imparo {
 

@@ -1,0 +1,543 @@
+// Picking a token per row of logits under a temperature, top-k, top-p and min-p, from a given random number per row.
+//
+// With m the largest logit of the row, T its temperature and w_i = exp((v_i - m) / T), the entries ordered by falling logit (equal
+// ones by rising index):
+//   K  the first top_k of the order (top_k <= 0: all)          P  the shortest beginning of K whose weight reaches top_p w(K)
+//   M  those of P with w_i >= min_p                            pick: the first index, in vocabulary order over M, at which the
+//                                                              running sum of w passes u w(M)
+// Every filter keeps a beginning of the same order, so the kept set is a cut (logit, index) and one more bound on the logit.
+//
+// Weights are whole numbers, w_i rounded to a multiple of 2^-shift (2^-45 for 131,072 entries), summed in 64 bits: sums are the
+// same whatever the order of their terms, so counts and sums may be gathered by atomics, part by part, and the picked index is the
+// one that 64-bit arithmetic gives except where a border lies within some 2^-40 of the drawn number.  In 32-bit sums, neighbours
+// with weights of 1e-5 of the total each were told apart wrongly once in some hundred rows.
+//
+// A cluster of CTAs owns a row, each CTA a contiguous stretch of it, which it keeps in shared memory: the row is read once.  The
+// cut is found by histograms over that copy (the cluster's CTAs exchange them through distributed shared memory): 1,024 bins of
+// equal width in (m - v) / T, the entries of the bin that holds the border sorted in shared memory; a bin with more entries than
+// the list holds is cut further by ten bits of the ordered logit at a time.
+#include "common.cuh"
+#include <cooperative_groups.h>
+
+namespace imparo {
+namespace sf {
+
+namespace cg = cooperative_groups;
+typedef unsigned long long u64;
+
+constexpr int THREADS = 512, WARPS = THREADS / 32;
+constexpr int BINS = 1024;                     // two per thread
+constexpr int LIST = 1024;                     // entries of a bin that are sorted at once
+constexpr int STAGED_MOST = 40960;             // entries of a stretch kept in shared memory (160 KB)
+constexpr float BIN_RANGE = 24.0f;             // (m - v) / T covered by the bins; the last one takes all beyond
+static_assert(BINS == 2 * THREADS && LIST == 2 * THREADS, "two bins and two list entries per thread");
+
+struct Args {
+    const void* logits;
+    const float* temperature;
+    const float* uniform;
+    const int* top_k;
+    const float* top_p;
+    const float* min_p;
+    int* out;
+    int* kept;
+    long long ld;
+    int vocab, per, shift;
+};
+
+struct Shared {
+    union {
+        struct { uint32_t n[BINS], lo[BINS], hi[BINS]; } own;      // this CTA's histogram: counts, weights in two halves
+        u64 list[LIST];                                            // entries of one bin, the same in every CTA of the cluster
+    };
+    uint32_t all_n[BINS];                                          // the cluster's histogram
+    u64 all_w[BINS];
+    double table[64];                                              // 2^(i / 64)
+    u64 warp_w[WARPS + 1];
+    uint32_t warp_n[WARPS + 1];
+    u64 part_top, part_w;                                          // read by the other CTAs
+    uint32_t part_n, list_n;
+    u64 before_w, found_cut;
+    uint32_t before_n, bin, found;
+};
+
+// a logit as a whole number of the same order, and back; equal logits have equal numbers (the zero's sign is dropped on loading)
+__device__ __forceinline__ uint32_t ordered(float v) {
+    const uint32_t u = __float_as_uint(v);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+// an entry's place in the order as one number: the larger comes first
+__device__ __forceinline__ u64 entry(float v, int index) { return ((u64)ordered(v) << 32) | (uint32_t)~index; }
+
+// NaN is no number: it is taken for minus infinity, which no filter keeps
+__device__ __forceinline__ float clean(float v) { return v == v ? v + 0.0f : -INFINITY; }
+
+struct Weights {
+    double top, rate;          // the row's largest logit; 64 log2(e) / T
+    const double* table;
+    float topf;
+    int shift;
+    // exp((v - top) / T) as a multiple of 2^-shift.  Table-driven exponential (P. T. P. Tang, 1989): t = 64 log2(e) (v - top) / T is
+    // split into a whole number n and a rest of at most 1/2; 2^(n / 64) from the table and the exponent, the rest by the first six
+    // terms of the series, |r| <= ln 2 / 128: what is left out is below 2^-54.
+    __device__ __forceinline__ u64 operator()(float v) const {
+        if (v == topf) return 1ull << shift;
+        const double t = ((double)v - top) * rate;
+        if (!(t > -64.0 * 64.0)) return 0;                         // below 2^-64 (and any number below an infinite one)
+        const double whole = 6755399441055744.0;                   // 1.5 2^52: adding it rounds to a whole number
+        const double tn = t + whole;
+        const int n = __double2loint(tn);
+        const double r = (t - (tn - whole)) * (0.69314718055994530942 / 64.0);
+        const double p = fma(r, fma(r, fma(r, fma(r, fma(r, 1.0 / 120.0, 1.0 / 24.0), 1.0 / 6.0), 0.5), 1.0), 1.0);
+        // times 2^(n >> 6) and 2^shift, by the exponent (at least 2^-64 2^44: a normal number)
+        const double scaled = table[n & 63] * p * __hiloint2double((1023 + (n >> 6) + shift) << 20, 0);
+        return __double_as_longlong(scaled + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;        // + 2^52: rounded to a whole number
+    }
+};
+
+// x times num for a float 0 <= x < 1, rounded down / up to a whole number
+__device__ __forceinline__ u64 part_of(float x, u64 num, bool up) {
+    const uint32_t bits = __float_as_uint(x);
+    const int e = (int)(bits >> 23);
+    const u64 mant = (bits & 0x7FFFFFu) | (e ? 0x800000u : 0u);
+    const int right = 150 - (e ? e : 1);                           // x = mant 2^-right, right >= 24 for x < 1
+    const u64 low = mant * num, high = __umul64hi(mant, num);
+    u64 q, rest;
+    if (right < 64) {
+        q = (high << (64 - right)) | (low >> right);               // high < 2^24 <= 2^right
+        rest = low & ((1ull << right) - 1);
+    } else if (right < 128) {
+        q = right == 64 ? high : high >> (right - 64);
+        rest = low | (right == 64 ? 0 : high & ((1ull << (right - 64)) - 1));
+    } else {
+        q = 0;
+        rest = low | high;
+    }
+    return q + (up && rest != 0 ? 1 : 0);
+}
+
+template <typename T>
+__device__ __forceinline__ float load1(const T* p) { return clean(to_f32(*p)); }
+
+template <typename V>
+__device__ __forceinline__ V warp_total(V v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// What comes before a thread's (n, w) in thread order.  All threads call it.
+__device__ __forceinline__ void block_before(Shared& s, uint32_t n, u64 w, uint32_t& before_n, u64& before_w) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t in = n;
+    u64 iw = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t un = __shfl_up_sync(0xffffffffu, in, o);
+        const u64 uw = __shfl_up_sync(0xffffffffu, iw, o);
+        if (lane >= o) { in += un; iw += uw; }
+    }
+    __syncthreads();
+    if (lane == 31) { s.warp_n[warp] = in; s.warp_w[warp] = iw; }
+    __syncthreads();
+    before_n = in - n;
+    before_w = iw - w;
+    for (int i = 0; i < warp; ++i) { before_n += s.warp_n[i]; before_w += s.warp_w[i]; }
+}
+
+// Sorts list[0 .. size) falling, size a power of two up to LIST.
+__device__ __forceinline__ void sort_list(u64* list, int size) {
+    for (int k = 2; k <= size; k <<= 1) {
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            __syncthreads();
+            const int i = threadIdx.x;
+            if (i < size / 2) {
+                const int a = 2 * j * (i / j) + i % j, b = a + j;
+                const u64 x = list[a], y = list[b];
+                if ((x < y) == ((a & k) == 0)) { list[a] = y; list[b] = x; }
+            }
+        }
+    }
+    __syncthreads();
+}
+
+template <typename T, bool STAGED>
+__global__ void __launch_bounds__(THREADS)
+sample_filtered_kernel(const Args a) {
+    extern __shared__ __align__(16) uint8_t sf_smem[];
+    Shared& s = *reinterpret_cast<Shared*>(sf_smem);
+    float* staged = reinterpret_cast<float*>(sf_smem + ((sizeof(Shared) + 15) & ~(size_t)15));
+    pdl_trigger();
+    pdl_wait();
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int r = blockIdx.x / ranks;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int lo = min(a.vocab, rank * a.per), count = min(a.vocab, lo + a.per) - lo;
+    const T* row = reinterpret_cast<const T*>(a.logits) + (size_t)r * a.ld + lo;
+    auto value = [&](int i) -> float { return STAGED ? staged[i] : load1(row + i); };
+
+    if (tid < 64) s.table[tid] = exp2((double)tid / 64.0);
+
+    // ---- the stretch into shared memory, its first largest entry ----
+    u64 top = 0;                                                   // (0: no number above minus infinity)
+    {
+        constexpr int VEC = 16 / sizeof(T);
+        int done = 0;
+        if (STAGED && ((uintptr_t)row & 15) == 0) {
+            const int vecs = count / VEC;
+            const uint4* src = reinterpret_cast<const uint4*>(row);
+#pragma unroll 4
+            for (int i = tid; i < vecs; i += THREADS) {
+                const uint4 raw = src[i];
+                const T* x = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float v = clean(to_f32(x[e]));
+                    staged[i * VEC + e] = v;
+                    if (v > -INFINITY) top = max(top, entry(v, lo + i * VEC + e));
+                }
+            }
+            done = vecs * VEC;
+        }
+        for (int i = done + tid; i < count; i += THREADS) {
+            const float v = load1(row + i);
+            if (STAGED) staged[i] = v;
+            if (v > -INFINITY) top = max(top, entry(v, lo + i));
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) s.warp_w[warp] = top;
+    __syncthreads();
+    if (tid == 0) {
+        for (int i = 1; i < WARPS; ++i) top = max(top, s.warp_w[i]);
+        s.part_top = top;
+    }
+    cluster.sync();
+    top = 0;
+    for (int i = 0; i < ranks; ++i) top = max(top, *cluster.map_shared_rank(&s.part_top, i));
+
+    const float temp = a.temperature[r];
+    if (top == 0 || !(temp > 0.f)) {                               // nothing to pick from, or greedy
+        if (rank == 0 && tid == 0) {
+            a.out[r] = top == 0 ? 0 : (int)~(uint32_t)top;
+            if (a.kept) a.kept[r] = top == 0 ? 0 : 1;
+        }
+        cluster.sync();                                            // no CTA ends while another reads its shared memory
+        return;
+    }
+    const float topf = unordered((uint32_t)(top >> 32));
+    Weights weight;
+    weight.top = topf; weight.topf = topf; weight.rate = 64.0 * 1.4426950408889634074 / (double)temp; weight.table = s.table;
+    weight.shift = a.shift;
+    const float per_bin = (float)BINS / (BIN_RANGE * temp);
+    // the bin of a logit: never falls as the logit falls, whatever the rounding
+    auto bin_of = [&](float v) -> int { return v == topf ? 0 : min(BINS - 1, (int)((topf - v) * per_bin)); };
+
+    // A histogram over the entries that `take` maps to a bin (-1: none), summed over the cluster into all_n (and all_w).
+    auto histogram = [&](bool weights, auto take) {
+        __syncthreads();
+        for (int i = tid; i < BINS; i += THREADS) { s.own.n[i] = 0; s.own.lo[i] = 0; s.own.hi[i] = 0; }
+        __syncthreads();
+        for (int i = tid; i < count; i += THREADS) {
+            const float v = value(i);
+            const int b = take(v, lo + i);
+            if (b >= 0) {
+                atomicAdd(&s.own.n[b], 1u);
+                if (weights) {
+                    const u64 w = weight(v);
+                    const uint32_t low = (uint32_t)w, old = atomicAdd(&s.own.lo[b], low);
+                    const uint32_t high = (uint32_t)(w >> 32) + (old + low < old ? 1u : 0u);
+                    if (high) atomicAdd(&s.own.hi[b], high);
+                }
+            }
+        }
+        cluster.sync();
+        const int share = BINS / ranks;                            // ranks is a power of two
+        for (int i = rank * share + tid; i < (rank + 1) * share; i += THREADS) {
+            uint32_t n = 0;
+            u64 w = 0;
+            for (int k = 0; k < ranks; ++k) {
+                const Shared* other = cluster.map_shared_rank(&s, k);
+                n += other->own.n[i];
+                if (weights) w += ((u64)other->own.hi[i] << 32) + other->own.lo[i];
+            }
+            for (int k = 0; k < ranks; ++k) {
+                Shared* other = cluster.map_shared_rank(&s, k);
+                other->all_n[i] = n;
+                other->all_w[i] = w;
+            }
+        }
+        cluster.sync();
+    };
+
+    // The cut behind the last entry kept: entries are counted (by_rank: the first `need` of the order stay) or weighed (those stay
+    // before which less than `need` weighs), over the entries at or above `least`.  whole_w: the weight of all of these.
+    auto find_cut = [&](bool by_rank, u64 least, float share_of_total) -> u64 {
+        u64 need = 0;
+        if (by_rank) need = (u64)a.top_k[r];
+        uint32_t before_n = 0;
+        u64 before_w = 0;
+        int chosen_bin = -1;                                       // the bin of equal width, then the prefix of the ordered logit
+        uint32_t prefix = 0;
+        for (int level = 0; ; ++level) {
+            // level 0: bins of equal width; levels 1 to 4: the next 10, 10, 10 and 2 bits of the ordered logit
+            const int down = level == 0 ? 32 : level < 4 ? 32 - 10 * level : 0, up = level == 1 ? 0 : 42 - 10 * level;
+            histogram(!by_rank, [&](float v, int index) -> int {
+                if (!(v > -INFINITY) || entry(v, index) < least) return -1;
+                const int b = bin_of(v);
+                if (level == 0) return b;
+                const uint32_t k = ordered(v);
+                if (b != chosen_bin || (level > 1 && (k >> (level == 4 ? 2 : up)) != prefix)) return -1;
+                return BINS - 1 - (int)((k >> down) & (level == 4 ? 3u : 1023u));
+            });
+            const uint32_t n0 = s.all_n[2 * tid], n1 = s.all_n[2 * tid + 1];
+            const u64 w0 = s.all_w[2 * tid], w1 = s.all_w[2 * tid + 1];
+            uint32_t bn;
+            u64 bw;
+            block_before(s, n0 + n1, w0 + w1, bn, bw);
+            if (level == 0) {
+                if (tid == THREADS - 1) { s.before_n = bn + n0 + n1; s.before_w = bw + w0 + w1; }
+                __syncthreads();
+                if (by_rank) {
+                    if (need >= s.before_n) return least;          // there are no more than top_k
+                } else {
+                    need = part_of(share_of_total, s.before_w, true);
+                    if (need == 0) need = 1;                       // the first entry always stays
+                }
+                __syncthreads();
+            }
+            // the first bin at whose end the count or the weight has been reached
+            bn += before_n;
+            bw += before_w;
+            const u64 at = by_rank ? bn : bw, x0 = by_rank ? n0 : w0, x1 = by_rank ? n1 : w1;
+            if (at < need && at + x0 >= need) { s.bin = 2 * tid; s.before_n = bn; s.before_w = bw; s.found = n0; }
+            else if (at + x0 < need && at + x0 + x1 >= need) { s.bin = 2 * tid + 1; s.before_n = bn + n0; s.before_w = bw + w0; s.found = n1; }
+            __syncthreads();
+            before_n = s.before_n;
+            before_w = s.before_w;
+            const int bin = (int)s.bin;
+            const uint32_t found = s.found;
+            if (level == 0) chosen_bin = bin;
+            else prefix = level == 4 ? prefix : (level == 1 ? 0u : prefix << 10) | (uint32_t)(BINS - 1 - bin);
+            const uint32_t last_digit = level == 4 ? (uint32_t)(BINS - 1 - bin) : 0u;
+            auto in_set = [&](float v, int index) -> bool {
+                if (!(v > -INFINITY) || entry(v, index) < least || bin_of(v) != chosen_bin) return false;
+                const uint32_t k = ordered(v);
+                if (level == 4) return k == ((prefix << 2) | last_digit);
+                return level == 0 || (k >> down) == prefix;
+            };
+            if (found <= LIST) {
+                // the bin's entries to every CTA of the cluster, sorted there
+                uint32_t mine = s.own.n[bin], first = 0;
+                for (int k = 0; k < rank; ++k) first += cluster.map_shared_rank(&s, k)->own.n[bin];
+                cluster.sync();                                    // the histograms are read: the list takes their place
+                if (tid == 0) s.list_n = first;
+                int size = 32;
+                while (size < (int)found) size <<= 1;
+                for (int i = (int)found + tid; i < size; i += THREADS) s.list[i] = 0;
+                __syncthreads();
+                if (mine) {
+                    for (int i = tid; i < count; i += THREADS) {
+                        const float v = value(i);
+                        if (in_set(v, lo + i)) {
+                            const uint32_t at_list = atomicAdd(&s.list_n, 1u);
+                            for (int k = 0; k < ranks; ++k) cluster.map_shared_rank(&s, k)->list[at_list] = entry(v, lo + i);
+                        }
+                    }
+                }
+                cluster.sync();
+                sort_list(s.list, size);
+                if (by_rank) return s.list[need - before_n - 1];
+                const int i0 = 2 * tid;
+                const u64 e0 = i0 < (int)found ? s.list[i0] : 0, e1 = i0 + 1 < (int)found ? s.list[i0 + 1] : 0;
+                const u64 v0 = e0 ? weight(unordered((uint32_t)(e0 >> 32))) : 0, v1 = e1 ? weight(unordered((uint32_t)(e1 >> 32))) : 0;
+                block_before(s, 0, v0 + v1, bn, bw);
+                bw += before_w;
+                // the last one before which less than `need` weighs
+                if (e1 && bw + v0 < need) atomicMax(&s.found, (uint32_t)(i0 + 1) + 0x40000000u);
+                else if (e0 && bw < need) atomicMax(&s.found, (uint32_t)i0 + 0x40000000u);
+                __syncthreads();
+                return s.list[s.found - 0x40000000u];
+            }
+            if (level == 4) {
+                // more equal logits than the list holds: the first so many by index
+                const float v = unordered((prefix << 2) | last_digit);
+                u64 stay;
+                if (by_rank) stay = need - before_n;
+                else {
+                    const u64 w = weight(v);
+                    stay = w ? min((u64)found, (need - before_w + w - 1) / w) : found;
+                }
+                const int seg = ((count + WARPS - 1) / WARPS + 31) / 32 * 32;
+                const int s0 = min(count, warp * seg), s1 = min(count, s0 + seg);
+                uint32_t n = 0;
+                for (int i = s0 + lane; i < s1; i += 32) n += in_set(value(i), lo + i) ? 1u : 0u;
+                n = warp_total(n);
+                __syncthreads();
+                if (lane == 0) s.warp_n[warp] = n;
+                __syncthreads();
+                if (tid == 0) {
+                    uint32_t total = 0;
+                    for (int i = 0; i < WARPS; ++i) total += s.warp_n[i];
+                    s.part_n = total;
+                    s.found_cut = 0;
+                }
+                cluster.sync();
+                u64 first = 0;
+                for (int k = 0; k < rank; ++k) first += cluster.map_shared_rank(&s, k)->part_n;
+                for (int i = 0; i < warp; ++i) first += s.warp_n[i];
+                if (first < stay && stay <= first + n) {           // this warp holds the last one that stays (warp-uniform)
+                    for (int i = s0 + lane; i - lane < s1; i += 32) {
+                        const bool is = i < s1 && in_set(value(i), lo + i);
+                        const unsigned mask = __ballot_sync(0xffffffffu, is);
+                        if (is && first + __popc(mask & ((2u << lane) - 1u)) == stay)
+                            for (int k = 0; k < ranks; ++k) cluster.map_shared_rank(&s, k)->found_cut = entry(v, lo + i);
+                        first += __popc(mask);
+                    }
+                }
+                cluster.sync();
+                return s.found_cut;
+            }
+        }
+    };
+
+    u64 cut = 1;                                                   // every number above minus infinity
+    if (a.top_k && a.top_k[r] > 0 && a.top_k[r] < a.vocab) cut = find_cut(true, cut, 0.f);
+    if (a.top_p && a.top_p[r] < 1.f) cut = find_cut(false, cut, a.top_p[r] > 0.f ? a.top_p[r] : 0.f);
+    if (a.min_p && a.min_p[r] > 0.f) {
+        // w >= min_p as a bound on the logit; above 1 only the first largest entry stays
+        const float p = a.min_p[r];
+        if (p > 1.f) cut = top;
+        else {
+            const float bound = __double2float_ru((double)topf + (double)temp * log((double)p));
+            if (bound > -INFINITY) cut = max(cut, (u64)ordered(bound + 0.0f) << 32);
+        }
+    }
+
+    // ---- the kept weights in vocabulary order: warps own contiguous stretches, whose sums are whole numbers ----
+    const int seg = ((count + WARPS - 1) / WARPS + 31) / 32 * 32;
+    const int s0 = min(count, warp * seg), s1 = min(count, s0 + seg);
+    u64 w = 0;
+    uint32_t n = 0;
+    for (int i = s0 + lane; i < s1; i += 32) {
+        const float v = value(i);
+        if (v > -INFINITY && entry(v, lo + i) >= cut) {
+            w += weight(v);
+            ++n;
+        }
+    }
+    w = warp_total(w);
+    n = warp_total(n);
+    __syncthreads();
+    if (lane == 0) { s.warp_w[warp] = w; s.warp_n[warp] = n; }
+    __syncthreads();
+    if (tid == 0) {
+        u64 tw = 0;
+        uint32_t tn = 0;
+        for (int i = 0; i < WARPS; ++i) { tw += s.warp_w[i]; tn += s.warp_n[i]; }
+        s.part_w = tw;
+        s.part_n = tn;
+    }
+    cluster.sync();
+    u64 before = 0, whole = 0;
+    uint32_t kept = 0;
+    for (int k = 0; k < ranks; ++k) {
+        const Shared* other = cluster.map_shared_rank(&s, k);
+        if (k < rank) before += other->part_w;
+        whole += other->part_w;
+        kept += other->part_n;
+    }
+    for (int i = 0; i < warp; ++i) before += s.warp_w[i];
+    const float u = a.uniform[r];
+    const u64 target = u < 1.f ? (u > 0.f ? part_of(u, whole, false) : 0) : whole - 1;       // the largest entry weighs: whole >= 1
+    if (before <= target && target < before + w) {                 // (warp-uniform) this warp holds the pick
+        for (int i = s0 + lane; i - lane < s1; i += 32) {
+            u64 x = 0;
+            if (i < s1) {
+                const float v = value(i);
+                if (v > -INFINITY && entry(v, lo + i) >= cut) x = weight(v);
+            }
+            u64 incl = x;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const u64 up = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += up;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, before + incl > target);
+            if (past) {
+                if (lane == __ffs(past) - 1) {
+                    a.out[r] = lo + i;
+                    if (a.kept) a.kept[r] = (int)kept;
+                }
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, incl, 31);
+        }
+    }
+    cluster.sync();
+}
+
+template <typename T>
+static int launch_sample(const Args& a, int n_rows, int ranks, bool staged, cudaStream_t stream) {
+    constexpr size_t fixed = (sizeof(Shared) + 15) & ~(size_t)15;
+    const size_t smem = fixed + (staged ? (size_t)a.per * sizeof(float) : 0);
+    auto kern = staged ? sample_filtered_kernel<T, true> : sample_filtered_kernel<T, false>;
+    // the attribute is the device's: set once on each
+    static bool configured[64][2] = {};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return (int)e;
+    if (device < 0 || device >= 64 || !configured[device][staged]) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(fixed + (staged ? STAGED_MOST * sizeof(float) : 0)));
+        if (e != cudaSuccess) return (int)e;
+        if (device >= 0 && device < 64) configured[device][staged] = true;
+    }
+    e = timeline_note(reinterpret_cast<const void*>(kern));
+    if (e != cudaSuccess) return (int)e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)n_rows * ranks);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ranks; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = imparo_pdl_enabled() ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, kern, a);
+    return e == cudaSuccess ? 0 : (int)e;
+}
+
+}  // namespace sf
+}  // namespace imparo
+
+using namespace imparo;
+
+// logits [n_rows, vocab] with row stride ld, float32 or bfloat16; temperature and uniform [n_rows]; top_k, top_p, min_p [n_rows] or
+// null; out [n_rows]; kept [n_rows] (how many entries the filters left) or null.
+extern "C" int imparo_sample_filtered(const void* logits, int dtype, long long ld, const float* temperature, const float* uniform,
+                                      const int* top_k, const float* top_p, const float* min_p, int* out, int* kept, int n_rows,
+                                      int vocab, cudaStream_t stream) {
+    if (n_rows <= 0) return 0;
+    if (!temperature || !uniform) return -7;
+    if (vocab < 1 || vocab > (1 << 24) || n_rows > (1 << 20) || ld < vocab) return -2;
+    if (dtype != IMPARO_DT_F32 && dtype != IMPARO_DT_BF16) return -1;
+    sf::Args a;
+    a.logits = logits; a.temperature = temperature; a.uniform = uniform; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p;
+    a.out = out; a.kept = kept; a.ld = ld; a.vocab = vocab;
+    int ranks = 1;
+    while (ranks < 8 && vocab > 2048 * ranks) ranks <<= 1;
+    a.per = ((vocab + ranks - 1) / ranks + 7) / 8 * 8;
+    // sums of vocab weights of at most 2^shift stay below 2^62
+    a.shift = 62;
+    while ((1ll << (62 - a.shift)) < vocab) --a.shift;
+    if (a.shift > 46) a.shift = 46;                                // (a weight is made as the low bits of a 52-bit number)
+    const bool staged = a.per <= sf::STAGED_MOST;
+    return dtype == IMPARO_DT_F32 ? sf::launch_sample<float>(a, n_rows, ranks, staged, stream)
+                                  : sf::launch_sample<__nv_bfloat16>(a, n_rows, ranks, staged, stream);
+}

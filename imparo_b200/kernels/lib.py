@@ -134,6 +134,9 @@ def _declare_kernels(lib):
     _declare(lib, "imparo_sgemm_cut_bytes", [I, I, I], c_int64)
     _declare(lib, "imparo_sgemm_cut", [P, P, P, I, I, I, I, I, I, P, P, S])
     _declare(lib, "imparo_sample_rows_parts", [P, P, P, P, P, P, I, I, I, S])
+    _declare(lib, "imparo_sample_filtered", [P, I, c_int64, P, P, P, P, P, P, P, I, I, S])
+    _declare(lib, "imparo_step_tables", [P, P, P, I, P, I, P, P, I, I, I, P, I, P, P, I, P, P, P, P, S])
+    _declare(lib, "imparo_attention_shared", [P, c_int64, P, P, I, P, P, P, I, I, I, I, P, P, I, I, c_float, P, P, P, P, I, I, I, I, I, I, I, I, P, S])
     _declare(lib, "imparo_take_sampled_tokens", [P, P, P, I, I, S])
     _declare(lib, "imparo_selftest_wait_limit", [P, I, P, S])
     _declare(lib, "imparo_zero_state_slots", [P, P, I, c_int64, P, I, I, P, S])

@@ -8,7 +8,7 @@ cobatch_rows.cuh:37-61).
 from __future__ import annotations
 
 import os
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -1559,6 +1559,157 @@ def sample_rows(logits, temperature, uniform, out) -> None:
             return
     _check(_lib.kernels().imparo_sample_rows(_ptr(logits), _ptr(temperature), _ptr(uniform), _ptr(out), n, vocab,
                                              logits.stride(0), _stream()), "sample_rows")
+
+
+def _here(what: str, *ts) -> None:
+    """All on the current device, whose stream the launch goes to."""
+    current = torch.cuda.current_device()
+    for t in ts:
+        _need(t is None or t.device.index == current, f"{what}: a tensor is on another device than the current one")
+
+
+def sample_filtered(logits, temperature, uniform, out, top_k=None, top_p=None, min_p=None, kept=None) -> None:
+    """out[r] = a token of row r of logits (float32 or bfloat16 [n, vocab], rows may be apart) drawn by uniform[r] in [0, 1) from
+    softmax(logits[r] / temperature[r]) after up to three filters, each a tensor with a value per row or None:
+
+    top_k (int32)    the k largest logits stay; 0 or less: all
+    top_p (float32)  of these the most likely ones stay, as few as reach top_p of their weight; 1 or more: all
+    min_p (float32)  of these the ones stay that are at least min_p times as likely as the most likely one; 0 or less: all
+
+    Equal logits stay by rising index; the most likely token always stays.  The pick is the first index, in vocabulary order over
+    what stays, at which the running sum passes uniform * total, in sums that are exact to 2^-38 or better of the largest weight.
+    temperature <= 0: the first maximum.  NaN counts as minus infinity, which is never picked; a row of nothing else gives 0.
+    kept (int32 or None): how many tokens the filters left (1 where greedy, 0 in a row of nothing).
+    temperature and uniform float32, out int32, all one value per row."""
+    _need(logits.is_cuda and logits.dim() == 2, "sample_filtered: logits [rows, vocab] on a CUDA device")
+    _cuda(temperature, uniform, out, top_k, top_p, min_p, kept)
+    _here("sample_filtered", logits, temperature, uniform, out, top_k, top_p, min_p, kept)
+    n, vocab = logits.shape
+    code = _code(logits)
+    _need(1 <= vocab <= 1 << 24 and n <= 1 << 20, "sample_filtered: 1 to 2^24 entries per row, at most 2^20 rows")
+    _need((vocab == 1 or logits.stride(1) == 1) and (n < 2 or logits.stride(0) >= vocab), "sample_filtered: a row's logits must lie side by side")
+    _need(temperature is not None and uniform is not None, "sample_filtered: temperature and uniform are needed")
+    for t, dtype, name in ((temperature, torch.float32, "temperature"), (uniform, torch.float32, "uniform"), (out, torch.int32, "out"),
+                           (top_k, torch.int32, "top_k"), (top_p, torch.float32, "top_p"), (min_p, torch.float32, "min_p"),
+                           (kept, torch.int32, "kept")):
+        _need(t is None or (t.dtype == dtype and t.numel() >= n), f"sample_filtered: {name} must be {dtype}, one value per row")
+    if n == 0:
+        return
+    _check(_lib.kernels().imparo_sample_filtered(_ptr(logits), code, logits.stride(0) if n > 1 else vocab, _ptr(temperature), _ptr(uniform),
+                                                 _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(out), _ptr(kept), n, vocab, _stream()),
+           "sample_filtered")
+
+
+def step_tables(lengths, counts, free_pages, held, page_size, n_pages, table, positions, item_of_token, row_start, slots, taken, status,
+                parent=None, shared=None) -> None:
+    """The description of a step made on the device.  Item r holds lengths[r] positions and brings counts[r] new tokens (int32 [items]).
+
+    table (int32 [items, blocks], written) is the step's block table: the row held[r] (int32 [items, any blocks], -1: no page), where
+    every block of the new positions that has no page takes the next one of free_pages (int32), items in order, blocks in order; -1
+    in all other blocks.  With parent and shared (int32 [items]): the first shared[r] // page_size blocks of an item whose parent[r] is
+    not -1 are those that held[parent[r]] lists; the page in which the shared positions end, if they end inside one, is the item's
+    own, and its shared part is for the caller to copy.
+    row_start (int32 [items + 1]): each item's first token, and their number.  positions, item_of_token (int32) and slots (int64, page *
+    page_size + place) per token; entries behind the last token get position -1 (which attends to nothing), item 0 and slot -1.
+    taken (int32 [1]): how many of the free pages are now in use.
+
+    A free list that is too short, a table or token arrays that are too narrow, negative lengths and pages outside [0, n_pages) are
+    recorded in the status word (read_status raises); nothing is written out of range, what has no page gets -1."""
+    _cuda(lengths, counts, free_pages, held, table, positions, item_of_token, row_start, slots, taken, status, parent, shared)
+    _here("step_tables", lengths, counts, free_pages, held, table, positions, item_of_token, row_start, slots, taken, status, parent, shared)
+    _need(held.dim() == 2 and table.dim() == 2 and held.shape[0] == table.shape[0], "step_tables: held and table must be [items, blocks]")
+    n, width = table.shape
+    for t, count, name in ((lengths, n, "lengths"), (counts, n, "counts"), (row_start, n + 1, "row_start"), (taken, 1, "taken"),
+                           (parent, n, "parent"), (shared, n, "shared"), (free_pages, 0, "free_pages"), (held, 0, "held"), (table, 0, "table"),
+                           (positions, 0, "positions"), (item_of_token, positions.numel(), "item_of_token"), (status, 4, "status")):
+        _need(t is None or (t.dtype == torch.int32 and t.numel() >= count), f"step_tables: {name} must be int32 with {count} entries at least")
+    _need(slots.dtype == torch.int64 and slots.numel() >= positions.numel(), "step_tables: slots must be int64, one per position")
+    _need((parent is None) == (shared is None), "step_tables: parent and shared go together")
+    _need(1 <= n <= 1 << 24 and width >= 1 and page_size >= 1 and n_pages >= 1, "step_tables: items, blocks, page size and pages")
+    _need(n_pages * page_size <= 1 << 40, "step_tables: slots of at most 2^40")
+    written = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (table, positions, item_of_token, row_start, slots, taken)]
+    for t in (held, free_pages, lengths, counts, parent, shared):
+        if t is not None and t.numel():
+            lo, hi = t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+            _need(all(hi <= a or b <= lo for a, b in written), "step_tables: what is read and what is written must not overlap")
+    _check(_lib.kernels().imparo_step_tables(_ptr(lengths), _ptr(counts), _ptr(free_pages), free_pages.numel(), _ptr(held), held.shape[1],
+                                             _ptr(parent), _ptr(shared), n, int(page_size), int(n_pages), _ptr(table), width,
+                                             _ptr(positions), _ptr(item_of_token), positions.numel(), _ptr(row_start), _ptr(slots),
+                                             _ptr(taken), _ptr(status), _stream()), "step_tables")
+
+
+class SharedPrefixPlan(NamedTuple):
+    """How paged_attention_shared cuts the keys, and the scratch it needs (float32 entries of part_acc and part_ml)."""
+    chunk_shared: int
+    n_shared: int
+    chunk_own: int
+    n_own: int
+    acc_floats: int
+    ml_floats: int
+
+
+def shared_prefix_plan(n_rows: int, n_groups: int, nh: int, nkv: int, hd: int, dtype: torch.dtype, most_shared: int, most_own: int,
+                       sms: Optional[int] = None) -> SharedPrefixPlan:
+    """A plan for rows of up to most_shared shared positions and most_own of their own.  A function of these sizes only; a longer
+    row is still attended to in full (the last stretch of keys takes what is left), it only takes longer."""
+    _need(n_rows >= 1 and n_groups >= 1 and nkv >= 1 and nh >= 1 and nh % nkv == 0, "shared_prefix_plan: rows, groups and heads")
+    _need(most_shared >= 0 and most_own >= 0, "shared_prefix_plan: lengths")
+    sms = sms if sms is not None else sm_count()
+    group = nh // nkv
+    tiles = -(-n_rows * group // 16) + n_groups - 1
+    n_shared = max(1, min(-(-most_shared // 64), -(-4 * sms // (nkv * tiles)), 256))
+    n_own = max(1, min(-(-most_own // 64), -(-4 * sms // (nkv * n_rows)), 64))
+    chunk_shared, chunk_own = (max(32, -(-(-(-most // n)) // 32) * 32) for most, n in ((most_shared, n_shared), (most_own, n_own)))
+    n_shared, n_own = max(1, -(-most_shared // chunk_shared)), max(1, -(-most_own // chunk_own))
+    parts = n_rows * nh * (n_shared + n_own)
+    return SharedPrefixPlan(chunk_shared, n_shared, chunk_own, n_own, parts * hd, parts * 2)
+
+
+def paged_attention_shared(q, k_cache, v_cache, positions, item_of_token, table, page_size, n_pages, group_start, shared_len, window, scale,
+                           out, part_acc, part_ml, plan: SharedPrefixPlan, nh, nkv, hd, status,
+                           sink_values: Optional[torch.Tensor] = None) -> None:
+    """paged_attention for rows that share their first positions: the rows group_start[g] .. group_start[g + 1] - 1 (int32 [groups + 1])
+    have the same keys and values at the positions 0 .. shared_len[g] - 1 (int32 [groups]), which are read once for all of them, by
+    the table row of the group's first row; the rest of each row's positions, up to its own, by its own table row, which lists all
+    of its pages as in paged_attention.  A group of one row and rows behind the last group are rows that share nothing.
+
+    q [rows, nh * hd] may be a slice of wider rows; out is dense.  float32 or bfloat16, head sizes that are multiples of 16 up to 256.
+    window: None, or the number of last positions a row sees.  A row of position -1 sees nothing and gives zeros.
+    sink_values (float32 [nh]): one more term exp(value) in each head's denominator.
+    plan: shared_prefix_plan() for these rows; part_acc and part_ml: the caller's scratch of plan.acc_floats and plan.ml_floats float32
+    entries, not to be shared by calls that may run at the same time."""
+    _need(q.is_cuda and q.dim() == 2 and (q.shape[1] == 1 or q.stride(1) == 1), "paged_attention_shared: q [rows, heads * head size], a row's values side by side")
+    tensors = (k_cache, v_cache, positions, item_of_token, table, group_start, shared_len, out, part_acc, part_ml, status, sink_values)
+    _cuda(*tensors)
+    _here("paged_attention_shared", q, *tensors)
+    T = q.shape[0]
+    _need(nkv >= 1 and nh % nkv == 0 and 16 <= hd <= 256 and hd % 16 == 0, "paged_attention_shared: heads, and head sizes of 16 to 256 in steps of 16")
+    _need(q.shape == (T, nh * hd) and out.shape == (T, nh * hd) and out.dtype == q.dtype, "paged_attention_shared: q/out shapes")
+    _need(k_cache.dtype == q.dtype and v_cache.dtype == q.dtype, "cache dtype must match q")
+    _need(page_size >= 1 and n_pages >= 1 and n_pages * page_size < 1 << 31, "paged_attention_shared: pages")
+    _need(min(k_cache.numel(), v_cache.numel()) >= n_pages * page_size * nkv * hd, "cache arena smaller than n_pages")
+    _need(table.dtype == torch.int32 and table.dim() == 2 and table.numel() > 0, "block table must be int32 [items, blocks]")
+    _need(positions.dtype == torch.int32 and item_of_token.dtype == torch.int32 and min(positions.numel(), item_of_token.numel()) >= T,
+          "positions / item_of_token must be int32 per row")
+    groups = shared_len.numel()
+    _need(groups >= 1 and group_start.numel() == groups + 1 and group_start.dtype == torch.int32 and shared_len.dtype == torch.int32,
+          "paged_attention_shared: group_start int32 [groups + 1], shared_len int32 [groups]")
+    _need(sink_values is None or (sink_values.dtype == torch.float32 and sink_values.numel() == nh), "sink values float32 [heads]")
+    _need(window is None or window >= 0, "paged_attention_shared: the window's size")
+    _need(plan.n_shared >= 1 and plan.n_own >= 1 and plan.n_shared + plan.n_own <= MAX_SPLITS, f"paged_attention_shared: 2 to {MAX_SPLITS} stretches of keys")
+    parts = T * nh * (plan.n_shared + plan.n_own)
+    _need(part_acc.dtype == torch.float32 and part_acc.numel() >= parts * hd and part_ml.dtype == torch.float32
+          and part_ml.numel() >= parts * 2, "paged_attention_shared: scratch too small for these rows and this plan")
+    _need(T <= 65535 and groups <= 65535, "paged_attention_shared: at most 65535 rows and groups per launch")
+    if T == 0:
+        return
+    code = _code(q)
+    _check(_lib.kernels().imparo_attention_shared(
+        _ptr(q), q.stride(0) if T > 1 else nh * hd, _ptr(k_cache), _ptr(v_cache), code, _ptr(positions), _ptr(item_of_token), _ptr(table),
+        table.shape[0], table.shape[1], int(page_size), int(n_pages), _ptr(group_start), _ptr(shared_len), groups, int(window or 0),
+        float(scale), _ptr(sink_values), _ptr(out), _ptr(part_acc), _ptr(part_ml), T, nh, nkv, hd, plan.chunk_shared, plan.n_shared,
+        plan.chunk_own, plan.n_own, _ptr(status), _stream()), "paged_attention_shared")
+    COUNTS["own"] += 1          # partial + combine
 
 
 # ---- stream operations of arrangements other than the pre-norm block (csrc/kernels/stream_ops.cu) ----------
