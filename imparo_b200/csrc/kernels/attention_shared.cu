@@ -9,90 +9,10 @@
 // stretch leaves, per row and head, the largest score, the sum of exp(score - largest) and the sum of the weighted values in 32-bit
 // (part_ml [rows, heads, splits, 2], part_acc [rows, heads, splits, head size], splits = n_shared + n_own), which the ordered combine
 // of attention_split.cu joins.
-#include "common.cuh"
+#include "attention_shared.cuh"
 
 namespace imparo {
 namespace sp {
-
-struct Args {
-    const void* q;
-    const void* k;
-    const void* v;
-    const int* positions;
-    const int* item_of_token;
-    const int* table;
-    const int* group_start;        // [n_groups + 1]
-    const int* shared;             // [n_groups]
-    float* part_acc;
-    float* part_ml;
-    int* status;
-    long long q_stride;            // elements between rows of q
-    int n_rows, n_items, n_groups, max_blocks, page_size, n_pages, window, nh, nkv, hd;
-    int chunk_shared, n_shared, chunk_own, n_own;
-    float scale;
-};
-
-// The rows [start, end) of a group and its shared positions, in range whatever the arrays hold.
-__device__ __forceinline__ void group_rows(const Args& a, int g, int& start, int& end) {
-    start = min(max(a.group_start[g], 0), a.n_rows);
-    end = min(max(a.group_start[g + 1], start), a.n_rows);
-}
-// the group a row belongs to, -1: none (the row then shares nothing)
-__device__ __forceinline__ int group_of(const Args& a, int t) {
-    int lo = 0, hi = a.n_groups;                                   // the last group that starts at or before t
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (a.group_start[mid] <= t) lo = mid + 1; else hi = mid;
-    }
-    const int g = lo - 1;
-    return g >= 0 && t < a.group_start[g + 1] ? g : -1;
-}
-__device__ __forceinline__ const int* table_row(const Args& a, int t, int kernel) {
-    const int item = a.item_of_token[t];
-    if (item < 0 || item >= a.n_items) {
-        report(a.status, IMPARO_ST_PAGE_RANGE, kernel, t, item);
-        return nullptr;
-    }
-    return a.table + (size_t)item * a.max_blocks;
-}
-__device__ __forceinline__ int first_seen(const Args& a, int pos) { return a.window > 0 && pos + 1 > a.window ? pos + 1 - a.window : 0; }
-
-// The keys [first, end) that the shared stretches take for a group: those of its shared positions that every row of it sees (rows
-// without a position, pos < 0, aside).  Each row takes the rest of what it sees, on both sides of them, with its own ones, so the
-// shared stretches need no mask by row and whatever a row does not see never meets its weights.  All threads call it; the result is
-// the same for every launch of the same arrays.
-struct Span { int first, end; };
-__device__ __forceinline__ Span shared_span(const Args& a, int g, int* scratch /* 2 */) {
-    if (g < 0) return Span{0, 0};                                  // (the same for the whole CTA)
-    if (threadIdx.x == 0) { scratch[0] = 0; scratch[1] = max(0, a.shared[g]); }
-    __syncthreads();
-    int start, end;
-    group_rows(a, g, start, end);
-    int lo = 0, hi = 0x7fffffff;
-    for (int t = start + threadIdx.x; t < end; t += blockDim.x) {
-        const int pos = a.positions[t];
-        if (pos >= 0) { lo = max(lo, first_seen(a, pos)); hi = min(hi, pos + 1); }
-    }
-    lo = __reduce_max_sync(0xffffffffu, lo);
-    hi = __reduce_min_sync(0xffffffffu, hi);
-    if ((threadIdx.x & 31) == 0) { atomicMax(&scratch[0], lo); atomicMin(&scratch[1], hi); }
-    __syncthreads();
-    const Span s{scratch[0], scratch[1]};
-    return s.first < s.end ? s : Span{0, 0};
-}
-// A row's own keys, counted through: the first `before` of them lie before the shared ones.
-struct Own {
-    int lo, before, skip, count;
-    __device__ __forceinline__ int key(int i) const { return lo + i + (i < before ? 0 : skip); }
-};
-__device__ __forceinline__ Own own_keys(const Args& a, int pos, Span s) {
-    Own o;
-    o.lo = first_seen(a, pos);
-    o.before = s.first < s.end ? s.first - o.lo : 0x7fffffff;      // (a row sees all of the span: lo <= first, end <= pos + 1)
-    o.skip = s.end - s.first;
-    o.count = pos < 0 ? 0 : pos + 1 - o.lo - o.skip;
-    return o;
-}
 
 // ---- any head size, 32-bit or bfloat16 -------------------------------------------------------------------------------
 // A CTA takes up to 16 rows (tokens of one group x query heads of one kv head) and one stretch of keys, 32 keys at a time in shared
@@ -301,7 +221,9 @@ extern "C" int imparo_attention_shared(const void* q, long long q_stride, const 
     a.n_rows = n_rows; a.n_items = n_items; a.n_groups = n_groups; a.max_blocks = max_blocks; a.page_size = page_size;
     a.n_pages = n_pages; a.window = window; a.nh = nh; a.nkv = nkv; a.hd = hd;
     a.chunk_shared = chunk_shared; a.n_shared = n_shared; a.chunk_own = chunk_own; a.n_own = n_own; a.scale = scale;
-    const int rc = dtype == IMPARO_DT_F32 ? sp::launch_any<float>(a, stream) : sp::launch_any<__nv_bfloat16>(a, stream);
+    int rc = dtype == IMPARO_DT_BF16 ? sp::launch_tc(a, out, sink_values, stream) : -8;
+    if (rc == 0 && n_own == 1) return 0;                     // its second kernel has joined everything
+    if (rc == -8) rc = dtype == IMPARO_DT_F32 ? sp::launch_any<float>(a, stream) : sp::launch_any<__nv_bfloat16>(a, stream);
     if (rc != 0) return rc;
     if (sink_values)
         return imparo_attention_split_combine_sinks(part_acc, part_ml, out, dtype, n_rows * nh, hd, n_shared + n_own, sink_values, nh, stream);

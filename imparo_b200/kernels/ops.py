@@ -1656,11 +1656,29 @@ def shared_prefix_plan(n_rows: int, n_groups: int, nh: int, nkv: int, hd: int, d
     _need(most_shared >= 0 and most_own >= 0, "shared_prefix_plan: lengths")
     sms = sms if sms is not None else sm_count()
     group = nh // nkv
-    tiles = -(-n_rows * group // 16) + n_groups - 1
-    n_shared = max(1, min(-(-most_shared // 64), -(-4 * sms // (nkv * tiles)), 256))
-    n_own = max(1, min(-(-most_own // 64), -(-4 * sms // (nkv * n_rows)), 64))
-    chunk_shared, chunk_own = (max(32, -(-(-(-most // n)) // 32) * 32) for most, n in ((most_shared, n_shared), (most_own, n_own)))
-    n_shared, n_own = max(1, -(-most_shared // chunk_shared)), max(1, -(-most_own // chunk_own))
+    if dtype == torch.bfloat16 and hd in (64, 128) and group <= 128:
+        # A CTA per SM takes up to two tiles of 128 rows through a stretch of 128-key steps; rows that fill one tile are taken by both,
+        # a step each.  The number of stretches is the one with the least time: rounds of CTAs, each as long as its steps and five
+        # more (what a CTA's start and end cost), and the partial results, written and read (in steps of 0.7 us at 6.5 TB/s).
+        tokens = 128 // group
+        each = -(-n_rows // n_groups)
+        ctas = nkv * n_groups * -(-each // (2 * tokens))
+        steps = max(1, -(-most_shared // 128))
+        per_step = 2 if each <= tokens else 1
+        cost = lambda n: -(-ctas * n // sms) * (-(-(-(-steps // n)) // per_step) + 5) + n * n_rows * nh * hd * 1.8e-6
+        n_shared = min(range(1, min(steps, 2 * sms) + 1), key=cost)
+        chunk_shared = -(-steps // n_shared) * 128
+        n_shared = -(-steps * 128 // chunk_shared)
+        # one stretch of own keys is joined with the shared ones at once; more only where few rows have long ones
+        n_own = max(1, min(-(-most_own // 512), -(-2 * sms // (n_rows * nkv * -(-group // 16))), 256))
+        chunk_own = max(64, -(-(-(-most_own // n_own)) // 64) * 64)
+        n_own = max(1, -(-most_own // chunk_own))
+    else:
+        tiles = -(-n_rows * group // 16) + n_groups - 1
+        n_shared = max(1, min(-(-most_shared // 64), -(-4 * sms // (nkv * tiles)), 256))
+        n_own = max(1, min(-(-most_own // 64), -(-4 * sms // (nkv * n_rows)), 64))
+        chunk_shared, chunk_own = (max(32, -(-(-(-most // n)) // 32) * 32) for most, n in ((most_shared, n_shared), (most_own, n_own)))
+        n_shared, n_own = max(1, -(-most_shared // chunk_shared)), max(1, -(-most_own // chunk_own))
     parts = n_rows * nh * (n_shared + n_own)
     return SharedPrefixPlan(chunk_shared, n_shared, chunk_own, n_own, parts * hd, parts * 2)
 
@@ -1709,7 +1727,7 @@ def paged_attention_shared(q, k_cache, v_cache, positions, item_of_token, table,
         table.shape[0], table.shape[1], int(page_size), int(n_pages), _ptr(group_start), _ptr(shared_len), groups, int(window or 0),
         float(scale), _ptr(sink_values), _ptr(out), _ptr(part_acc), _ptr(part_ml), T, nh, nkv, hd, plan.chunk_shared, plan.n_shared,
         plan.chunk_own, plan.n_own, _ptr(status), _stream()), "paged_attention_shared")
-    COUNTS["own"] += 1          # partial + combine
+    COUNTS["own"] += 1          # (the stretches, and what joins them)
 
 
 # ---- stream operations of arrangements other than the pre-norm block (csrc/kernels/stream_ops.cu) ----------
