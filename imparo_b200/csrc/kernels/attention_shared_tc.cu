@@ -13,36 +13,38 @@ namespace sp {
 using namespace tc;
 
 // ---- the shared keys ---------------------------------------------------------------------------------------------------
-// One CTA per SM, 128 keys a step:
-//   warps 0-3, 4-7  the softmax of tile A and B, one thread per row (= tensor-memory lane): the row's 128 scores of the step go into
-//                   registers at once, P = exp2(s - max) goes back to tensor memory as bfloat16, where the second product reads it
-//   warp 8          TMA: keys and values page by page (lane p fetches page p of a step) into rings with barriers of their own
-//   warps 9, 10     tcgen05.mma, one issuing thread per tile: S = Q K^T (both from shared memory), O += P V (P from tensor memory)
+// One CTA per SM, 64 keys a step, TILES tiles of 128 rows (four with head size 64, two with 128: what tensor memory holds):
+//   4 warps a tile  the softmax, one thread per row (= tensor-memory lane): the row's 64 scores of the step go into registers at once,
+//                   P = exp2(s - max) goes back to their columns as bfloat16, where the second product reads it
+//   1 warp          TMA: keys and values page by page (lane p fetches page p of a step) into rings with barriers of their own
+//   2 warps         tcgen05.mma, each for every other tile: S = Q K^T (both from shared memory), O += P V (P from tensor memory)
 // The output stays in tensor memory; it is scaled down only when a row's max has grown by more than 8 (in log2 units) since the max
 // in use was taken, which leaves every term below 2^8 and the result the same.
-// With head size 64 P has columns of its own, and the next step's scores are computed while this step's are weighted.  With 128 the
-// scores' own columns take P; the other tile's softmax runs while this tile's products do.
-// A group's rows that fill one tile at most are given to both: A takes the even steps, B the odd ones, and A adds B's result at the
-// end (otherwise the SM's exponential units would wait for one tile's products every step).
-constexpr int TILE = 128, STEP = 128;              // rows per tile, keys per step
-constexpr int TC_THREADS = 384, LOAD_WARP = 8, MMA_WARP = 9;
-constexpr uint32_t REGION = 128 * 128;             // a [128 rows][64 dims] block in shared memory
+// Rows that fill one or two tiles only are given to all of them: of P tiles with the same rows, each takes every P-th step, and the
+// first one adds the others' results at the end.
+constexpr int TILE = 128, STEP = 64;               // rows per tile, keys per step
+constexpr uint32_t REGION = TILE * 128;            // [128 rows][64 dims] of queries in shared memory
+constexpr uint32_t KEY_REGION = STEP * 128;        // [64 keys][64 dims] of keys or values
 constexpr float GROW = 8.0f;
 constexpr float LN2 = 0.69314718055994530942f, LOG2E = 1.4426950408889634074f;
 
 template <int HD> struct Shape {
     static constexpr int NB = HD / 64;                       // 64-dim blocks of a head
-    static constexpr int STAGES = HD == 64 ? 4 : 2;          // even: where the tiles take turns at the steps, a buffer is always the same tile's
-    static constexpr bool ALIAS = HD == 128;                 // P in the scores' columns
-    static constexpr uint32_t BLOCK = NB * REGION;           // a tile of queries, a step's keys or its values
-    static constexpr uint32_t S_COL = 0, O_COL = 256, P_COL = ALIAS ? 0 : 384, P_STRIDE = ALIAS ? 128 : 64;
-    static constexpr size_t SMEM = 1024 + 2 * BLOCK + (size_t)STAGES * 2 * BLOCK + 512;
+    static constexpr int TILES = HD == 64 ? 4 : 2;
+    static constexpr int S_BUFS = HD == 64 ? 1 : 2;          // steps whose scores a tile holds at once
+    static constexpr int STAGES = HD == 64 ? 8 : 4;          // a multiple of TILES: a buffer always holds steps of the same tiles
+    static constexpr int LOAD_WARP = 4 * TILES, MMA_WARP = LOAD_WARP + 1, THREADS = 32 * (LOAD_WARP + 3);
+    static constexpr uint32_t Q_BYTES = NB * REGION, KEY_BYTES = NB * KEY_REGION;
+    static constexpr uint32_t O_COL = TILES * S_BUFS * STEP;                 // tensor memory: scores (and P) first, then outputs
+    static_assert(O_COL + TILES * HD == 512 && STAGES % TILES == 0, "tensor memory and stages");
+    static constexpr int PAGES = 4096, REFILL = 1024;        // the copies' rows of the cache: a ring, filled so many at a time
+    static constexpr size_t SMEM = 1024 + TILES * Q_BYTES + (size_t)STAGES * 2 * KEY_BYTES + 512 + PAGES * 4;
 };
 
 __device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {           // values: [key][dim], the dims contiguous (MN-major)
     uint64_t d = 0;
     d |= (uint64_t)((addr & 0x3FFFF) >> 4);
-    d |= (uint64_t)((REGION >> 4) & 0x3FFF) << 16;                     // 64-dim blocks
+    d |= (uint64_t)((KEY_REGION >> 4) & 0x3FFF) << 16;                 // 64-dim blocks
     d |= (uint64_t)(1024 >> 4) << 32;                                  // groups of 8 keys
     d |= (uint64_t)1 << 46;
     d |= (uint64_t)2 << 61;
@@ -56,18 +58,61 @@ __device__ __forceinline__ void umma_ta(uint32_t d, uint32_t a, uint64_t b, uint
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
                  ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate) : "memory");
 }
+// One lane of a warp that is together.  The instructions of the tensor cores take their operands from registers that the whole warp
+// shares: in the branch of an elected lane the compiler knows that there is one such value, in one on the lane's number it does not.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+    return one != 0;
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+// 2^x for two numbers x <= 8 on the multiply-add units, which have time where the exponential units have none: 2^x = 2^n 2^f, n whole,
+// |f| <= 1/2, and the cubic for 2^f whose largest relative error on that range is the least a cubic can have (7.5e-5, a fortieth of
+// the step of the bfloat16 that takes the result).  Adding 1.5 2^23 rounds to a whole number, which then lies in the low bits.
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+    const float2 whole = make_float2(12582912.f, 12582912.f);
+    x.x = fmaxf(x.x, -126.f);
+    x.y = fmaxf(x.y, -126.f);
+    const float2 n = __fadd2_rn(x, whole);
+    const float2 f = __fadd2_rn(x, __fadd2_rn(whole, make_float2(-n.x, -n.y)));
+    float2 p = __ffma2_rn(f, make_float2(0.05517165735f, 0.05517165735f), make_float2(0.24261112511f, 0.24261112511f));
+    p = __ffma2_rn(f, p, make_float2(0.69326096773f, 0.69326096773f));
+    p = __ffma2_rn(f, p, make_float2(0.99992805719f, 0.99992805719f));
+    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(n.x) << 23)),
+                       __int_as_float(__float_as_int(p.y) + (__float_as_int(n.y) << 23)));
+}
+#ifndef SP_FMA
+#define SP_FMA 0
+#endif
+// the largest of three; no number if one of them is none
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
 }
-__device__ __forceinline__ void arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// false when the wait ran out
+__device__ __forceinline__ bool wait_at(uint32_t bar, uint32_t parity) {
+    for (uint32_t it = 0; it < WAIT_LIMIT; ++it) {
+        uint32_t done;
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.b32 %0, 1, 0, p;\n}"
+                     : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        if (done) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ void commit_at(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -90,54 +135,55 @@ __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <int HD>
-__global__ void __launch_bounds__(TC_THREADS, 1)
+__global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
 shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Args a, const int n_splits) {
     using C = Shape<HD>;
-    constexpr int NB = C::NB, ST = C::STAGES;
+    constexpr int NB = C::NB, ST = C::STAGES, NT = C::TILES, SB = C::S_BUFS;
     extern __shared__ __align__(1024) uint8_t tc_smem_raw[];
     __shared__ int span_scratch[2];
     uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)tc_smem_raw + 1023) & ~(uintptr_t)1023);
-    uint8_t* q_s = smem;                                     // [2][BLOCK]
-    uint8_t* k_s = q_s + 2 * C::BLOCK;                       // [ST][BLOCK]
-    uint8_t* v_s = k_s + ST * C::BLOCK;                      // [ST][BLOCK]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + ST * C::BLOCK);
+    uint8_t* q_s = smem;                                     // [NT][Q_BYTES]
+    uint8_t* k_s = q_s + NT * C::Q_BYTES;                    // [ST][KEY_BYTES]
+    uint8_t* v_s = k_s + ST * C::KEY_BYTES;                  // [ST][KEY_BYTES]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + ST * C::KEY_BYTES);
     uint64_t* k_full = bars;                                 // [ST]
     uint64_t* k_empty = k_full + ST;
     uint64_t* v_full = k_empty + ST;
     uint64_t* v_empty = v_full + ST;
-    uint64_t* q_ready = v_empty + ST;                        // [2]
-    uint64_t* s_ready = q_ready + 2;                         // [2]  the tile's scores of a step are complete
-    uint64_t* s_free = s_ready + 2;                          // [2]  ... and have been read into registers
-    uint64_t* p_half = s_free + 2;                           // [2]  the first 64 keys' weights are written, the output is scaled
-    uint64_t* p_ready = p_half + 2;                          // [2]  all are
-    uint64_t* o_done = p_ready + 2;                          // [2]  P V of the step is accumulated
-    uint64_t* drained = o_done + 2;                          // [2]  every product of the tile has run
+    uint64_t* q_ready = v_empty + ST;                        // [NT]
+    uint64_t* s_ready = q_ready + NT;                        // [NT][SB] the tile's scores of a step are complete
+    uint64_t* p_ready = s_ready + NT * SB;                   // [NT] the step's weights are written, the output is scaled
+    uint64_t* o_done = p_ready + NT;                         // [NT] P V of the step is accumulated (with one buffer of scores: of the last step)
+    uint64_t* drained = o_done + NT;                         // [2]  every product of an issuing warp has run
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 2);
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    static_assert((4 * 5 + 14) * 8 + 8 <= 512, "barriers");
+    static_assert((4 * ST + NT * (3 + SB) + 2) * 8 + 8 <= 512, "barriers");
 
     timeline_begin();
     pdl_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int G = a.nh / a.nkv, TQ = TILE / G;               // tokens per tile
     const int kvh = blockIdx.x, chunk = blockIdx.y;
     int group = 0, unit = blockIdx.z, start = 0, end = 0;
     for (; group < a.n_groups; ++group) {
         group_rows(a, group, start, end);
-        const int units = (end - start + 2 * TQ - 1) / (2 * TQ);
+        const int units = (end - start + NT * TQ - 1) / (NT * TQ);
         if (unit < units) break;
         unit -= units;
     }
     if (group >= a.n_groups) return;                         // the grid is an upper bound (uniform per CTA)
-    const int row0 = start + unit * 2 * TQ, n_tok = min(2 * TQ, end - row0);
-    const bool both = n_tok <= TQ;                           // one tile of rows, which both halves of the CTA work on
+    const int row0 = start + unit * NT * TQ, n_tok = min(NT * TQ, end - row0);
+    const int row_tiles = (n_tok + TQ - 1) / TQ;
+    const int log_r = row_tiles > 2 ? 2 : row_tiles - 1, R = 1 << log_r;   // tile x: rows x % R, every phases-th step from x / R on
+    const int phases = NT >> log_r;
+    const int n_tiles = R > 2 ? row_tiles : NT;              // (a fourth tile without rows does nothing)
     const Span span = shared_span(a, group, span_scratch);
     const int per_chunk = a.chunk_shared / STEP;
     const int first_step = span.first / STEP + chunk * per_chunk;
     const int all_steps = (span.end + STEP - 1) / STEP;
     const int n_steps = span.first < span.end ? max(0, (chunk + 1 < a.n_shared ? min(all_steps, first_step + per_chunk) : all_steps) - first_step) : 0;
     if (n_steps == 0) {
-        for (int i = threadIdx.x; i < n_tok * G; i += TC_THREADS) {
+        for (int i = threadIdx.x; i < n_tok * G; i += C::THREADS) {
             float* ml = a.part_ml + (((size_t)(row0 + i / G) * a.nh + kvh * G + i % G) * n_splits + chunk) * 2;
             ml[0] = -INFINITY;
             ml[1] = 0.f;
@@ -146,19 +192,21 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
 
     if (threadIdx.x == 0) {
-        const int readers = both ? 1 : 2;                    // a step's keys and values are free when every tile that uses them has read them
+        const int readers = min(R, row_tiles);               // a step's keys and values are free when all tiles that use them have read them
         for (int s = 0; s < ST; ++s) {
             mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], readers);
             mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], readers);
         }
-        for (int x = 0; x < 2; ++x) {
-            mbar_init(&q_ready[x], 128); mbar_init(&s_ready[x], 1); mbar_init(&s_free[x], 128);
-            mbar_init(&p_half[x], 128); mbar_init(&p_ready[x], 128); mbar_init(&o_done[x], 1); mbar_init(&drained[x], 1);
+        for (int x = 0; x < NT; ++x) {
+            mbar_init(&q_ready[x], 128); mbar_init(&p_ready[x], 128); mbar_init(&o_done[x], 1);
+            for (int i = 0; i < SB; ++i) mbar_init(&s_ready[x * SB + i], 1);
         }
+        mbar_init(&drained[0], 1);
+        mbar_init(&drained[1], 1);
         *gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == MMA_WARP) {
+    if (warp == C::MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -168,34 +216,47 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     // The next kernel may start now: everything before this one is complete (it reads what those wrote before it waits for this
     // one), and this CTA has its tensor memory, which no later kernel's CTA can hold any more while it waits for this one.
     pdl_trigger_late();
-    const uint32_t tmem = *tmem_slot;
-    // tile x works on steps at(0), at(1), ... of the CTA's
-    auto steps_of = [&](int x) { return both ? (n_steps + 1 - x) >> 1 : n_steps; };
-    auto at = [&](int x, int j) { return both ? 2 * j + x : j; };
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    // tile x works on the steps at(x, 0), at(x, 1), ... of the CTA's
+    auto steps_of = [&](int x) { return x < n_tiles ? (n_steps - (x >> log_r) + phases - 1) / phases : 0; };
+    auto at = [&](int x, int j) { return j * phases + (x >> log_r); };
 
-    if (warp == LOAD_WARP) {
-        // keys and values are fetched as their buffers come free, whichever first
+    if (warp == C::LOAD_WARP) {
+        // Keys and values are fetched as their buffers come free, whichever first.  Where the copies' rows lie is looked up a
+        // thousand copies at a time: a lookup per copy is a trip to memory that every step then waits for.
+        int* where = reinterpret_cast<int*>(bars + 64);      // [PAGES] first cache row of copy c of the CTA's, at c % PAGES
         const int* tab = table_row(a, start, 72);
-        const int box = min(a.page_size, STEP), copies = STEP / box;
+        const int box = min(a.page_size, STEP), log_copies = box == 16 ? 2 : box == 32 ? 1 : 0, copies = 1 << log_copies;
         const int first_blk = span.first / a.page_size, last_blk = (span.end - 1) / a.page_size;
-        auto load = [&](int i, bool values) {                // warp-uniform call
-            const int s = i % ST;
-            uint8_t* dst = (values ? v_s : k_s) + s * C::BLOCK;
-            uint64_t* bar = values ? &v_full[s] : &k_full[s];
-            if (lane == 0) mbar_expect_tx(bar, C::BLOCK);
-            __syncwarp();
-            for (int c = lane; c < copies; c += 32) {
+        int known = 0;
+        auto look_up = [&]() {
+            const int until = min(known + C::REFILL, n_steps << log_copies);
+            for (int c = known + lane; c < until; c += 32) {
                 // blocks in which nothing is seen: a page that is seen stands in for them (its values are cleared below)
-                const int key = (first_step + i) * STEP + c * box, blk = min(max(key / a.page_size, first_blk), last_blk);
+                const int key = first_step * STEP + c * box, blk = min(max(key / a.page_size, first_blk), last_blk);
                 int page = tab != nullptr && blk < a.max_blocks ? tab[blk] : -1;
                 if (page < 0 || page >= a.n_pages) {
                     report(a.status, IMPARO_ST_PAGE_RANGE, 73, start, page);
                     page = 0;
                 }
-                const int y = page * a.page_size + key % a.page_size;
+                where[c % C::PAGES] = page * a.page_size + key % a.page_size;
+            }
+            known = until;
+            __syncwarp();
+        };
+        look_up();
+        auto load = [&](int i, bool values) {                // warp-uniform call
+            const int s = i % ST;
+            uint8_t* dst = (values ? v_s : k_s) + s * C::KEY_BYTES;
+            uint64_t* bar = values ? &v_full[s] : &k_full[s];
+            if (!values && (i + 1) << log_copies > known) look_up();         // (values follow their keys by a few steps)
+            if (lane == 0) mbar_expect_tx(bar, C::KEY_BYTES);
+            __syncwarp();
+            if (lane < copies) {
+                const int y = where[((i << log_copies) + lane) % C::PAGES];
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
-                    tma_load_2d(dst + nb * REGION + (uint32_t)c * box * 128, values ? &map_v : &map_k, bar, kvh * HD + nb * 64, y);
+                    tma_load_2d(dst + nb * KEY_REGION + (uint32_t)lane * box * 128, values ? &map_v : &map_k, bar, kvh * HD + nb * 64, y);
             }
         };
         int k_next = 0, v_next = 0;
@@ -204,7 +265,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             int what = 0;                                    // bit 0: the next keys' buffer is free, bit 1: the next values', bit 2: stop
             if (lane == 0) {
                 if (k_next < n_steps && (k_next < ST || mbar_test(&k_empty[k_next % ST], ((k_next / ST) - 1) & 1))) what |= 1;
-                if (v_next < n_steps && (v_next < ST || mbar_test(&v_empty[v_next % ST], ((v_next / ST) - 1) & 1))) what |= 2;
+                if (v_next < k_next && (v_next < ST || mbar_test(&v_empty[v_next % ST], ((v_next / ST) - 1) & 1))) what |= 2;
                 if (*gave_up) what = 4;
                 if (what == 0 && ++idle > WAIT_LIMIT / 16) {
                     report(a.status, IMPARO_ST_WAIT_LIMIT, 74, k_next, v_next);
@@ -223,233 +284,259 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             for (int i = max(0, k_next - ST); i < k_next; ++i) mbar_wait(&k_full[i % ST], (i / ST) & 1);
             for (int i = max(0, v_next - ST); i < v_next; ++i) mbar_wait(&v_full[i % ST], (i / ST) & 1);
         }
-    } else if (warp == MMA_WARP || warp == MMA_WARP + 1) {
-        const int x = warp - MMA_WARP, n_x = steps_of(x);
-        const uint64_t qd = smem_desc(smem_u32(q_s + x * C::BLOCK)), kd0 = smem_desc(smem_u32(k_s)), vd0 = desc_mn(smem_u32(v_s));
+    } else if (warp >= C::MMA_WARP) {
+        constexpr int MINE = NT / 2;                         // this warp's tiles: w, w + 2
+        const int w = warp - C::MMA_WARP;
+        const uint64_t qd0 = smem_desc(smem_u32(q_s)), kd0 = smem_desc(smem_u32(k_s)), vd0 = desc_mn(smem_u32(v_s));
         const uint32_t id_s = idesc(STEP, false), id_o = idesc(HD, true);
-        const uint32_t t_s = tmem + C::S_COL + x * 128, t_o = tmem + C::O_COL + x * HD, t_p = tmem + C::P_COL + x * C::P_STRIDE;
-        auto wait = [&](uint64_t* bar, uint32_t parity, int code, int j) -> bool {       // the whole warp
-            int good = 1;
-            if (lane == 0 && !mbar_wait(bar, parity)) {
-                report(a.status, IMPARO_ST_WAIT_LIMIT, code, j, x);
+        const uint32_t b_kf = smem_u32(k_full), b_ke = smem_u32(k_empty), b_vf = smem_u32(v_full), b_ve = smem_u32(v_empty),
+                       b_s = smem_u32(s_ready), b_p = smem_u32(p_ready), b_o = smem_u32(o_done);
+        bool ok = true;
+        auto wait = [&](uint32_t bar, uint32_t parity, int code, int j) {                // the whole warp
+            if (!wait_at(bar, parity)) {
+                report(a.status, IMPARO_ST_WAIT_LIMIT, code, j, w);
                 *gave_up = 1;
-                good = 0;
+                ok = false;
             }
-            good = __shfl_sync(0xffffffffu, good, 0);
-            fence_after();
-            return good != 0;
+            ok = __all_sync(0xffffffffu, ok);
         };
-        auto issue_s = [&](int j) {                          // S = Q K^T of the tile's step j
-            if (lane == 0) {
-                const int s = at(x, j) % ST;
-                const uint64_t kd = kd0 + (uint64_t)((s * C::BLOCK) >> 4);
+        int k_seen = -1, v_seen = -1;                        // the last step whose keys / values this warp has waited for
+        auto scores = [&](int x, int j) {                    // S = Q K^T of the tile's step j
+            const int i = at(x, j), s = i % ST;
+            if (i != k_seen) { wait(b_kf + s * 8, (i / ST) & 1, 76, i); k_seen = i; }
+            if (!ok) return;
+            if (elect_one()) {
+                const uint64_t qd = qd0 + (uint64_t)(((x & (R - 1)) * C::Q_BYTES) >> 4), kd = kd0 + (uint64_t)((s * C::KEY_BYTES) >> 4);
+                const uint32_t t_s = tmem + (x * SB + j % SB) * STEP;
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                     for (int k = 0; k < BK / UMMA_K; ++k)
-                        umma(t_s, qd + (uint64_t)((nb * REGION + k * 32) >> 4), kd + (uint64_t)((nb * REGION + k * 32) >> 4), id_s,
+                        umma(t_s, qd + (uint64_t)((nb * REGION + k * 32) >> 4), kd + (uint64_t)((nb * KEY_REGION + k * 32) >> 4), id_s,
                              (nb > 0 || k > 0) ? 1u : 0u);
-                umma_commit(&s_ready[x]);
-                umma_commit(&k_empty[s]);
-            }
-            __syncwarp();
-        };
-        auto issue_pv = [&](int j, int half) {               // O += P V over 64 keys of the step
-            if (lane == 0) {
-                const int s = at(x, j) % ST;
-                const uint64_t vd = vd0 + (uint64_t)((s * C::BLOCK) >> 4);
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int kk = half * 4 + u;
-                    umma_ta(t_o, t_p + kk * 8, vd + (uint64_t)((kk * (UMMA_K * 128)) >> 4), id_o, (kk > 0 || j > 0) ? 1u : 0u);
-                }
-                if (half == 1) {
-                    umma_commit(&o_done[x]);
-                    umma_commit(&v_empty[s]);
-                }
+                commit_at(b_s + (x * SB + j % SB) * 8);
+                commit_at(b_ke + s * 8);
             }
             __syncwarp();
         };
         // values outside the span are cleared: their weights are 0, and what lies there may be infinite or no number
-        auto clear_values = [&](int j) {
-            const int key0 = (first_step + at(x, j)) * STEP, lo = max(0, span.first - key0), hi = min(STEP, span.end - key0);
-            if (lo == 0 && hi == STEP) return;
-            uint8_t* v = v_s + (at(x, j) % ST) * C::BLOCK;
-            for (int i = lane; i < STEP * NB * 8; i += 32) {
-                const int row = (i >> 3) % STEP, nb = (i >> 3) / STEP;
-                if (row < lo || row >= hi) *reinterpret_cast<uint4*>(v + nb * REGION + row * 128 + (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        const int clear_first = span.first % STEP != 0 && chunk == 0 ? 0 : -1;
+        const int clear_last = span.end % STEP != 0 && first_step + n_steps == all_steps ? n_steps - 1 : -1;
+        auto clear_values = [&](int i) {
+            const int key0 = (first_step + i) * STEP, lo = max(0, span.first - key0), hi = min(STEP, span.end - key0);
+            uint8_t* v = v_s + (i % ST) * C::KEY_BYTES;
+            for (int c = lane; c < STEP * NB * 8; c += 32) {
+                const int row = (c >> 3) % STEP, nb = (c >> 3) / STEP;
+                if (row < lo || row >= hi) *reinterpret_cast<uint4*>(v + nb * KEY_REGION + row * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
         };
-        auto full = [&](uint64_t* bar, int j, int code) { const int i = at(x, j); return wait(&bar[i % ST], (i / ST) & 1, code, j); };
-        bool ok = n_x > 0 && wait(&q_ready[x], 0, 75, 0) && full(k_full, 0, 76);
-        if (ok) issue_s(0);
-        for (int j = 0; j < n_x && ok; ++j) {
-            if (!C::ALIAS && j + 1 < n_x) {
-                ok = wait(&s_free[x], j & 1, 77, j) && full(k_full, j + 1, 76);
-                if (!ok) break;
-                issue_s(j + 1);
+        int n_x[MINE];
+#pragma unroll
+        for (int u = 0; u < MINE; ++u) {
+            const int x = w + 2 * u;
+            n_x[u] = steps_of(x);
+            if (n_x[u] > 0 && ok) {
+                wait(smem_u32(&q_ready[x & (R - 1)]), 0, 75, x);
+                fence_after();
             }
-            ok = full(v_full, j, 78);
-            if (!ok) break;
-            clear_values(j);
-            ok = wait(&p_half[x], j & 1, 79, j);
-            if (!ok) break;
-            issue_pv(j, 0);
-            ok = wait(&p_ready[x], j & 1, 80, j);
-            if (!ok) break;
-            issue_pv(j, 1);
-            if (C::ALIAS && j + 1 < n_x) {                   // (behind P V in the tensor cores' order, which reads the same columns)
-                ok = full(k_full, j + 1, 76);
-                if (!ok) break;
-                issue_s(j + 1);
+            for (int j = 0; j < SB && j < n_x[u] && ok; ++j) scores(x, j);
+        }
+        for (int j = 0; j < n_x[0] && ok; ++j) {             // (a later tile has no more steps than an earlier one)
+#pragma unroll
+            for (int u = 0; u < MINE; ++u) {
+                const int x = w + 2 * u, i = at(x, j), s = i % ST;
+                if (j >= n_x[u] || !ok) continue;
+                if (i != v_seen) {
+                    wait(b_vf + s * 8, (i / ST) & 1, 78, i);
+                    if (!ok) continue;
+                    v_seen = i;
+                    if (i == clear_first || i == clear_last) clear_values(i);
+                }
+                wait(b_p + x * 8, j & 1, 79, j);
+                if (!ok) continue;
+                fence_after();
+                if (elect_one()) {                           // O += P V
+                    const uint64_t vd = vd0 + (uint64_t)((s * C::KEY_BYTES) >> 4);
+                    const uint32_t t_p = tmem + (x * SB + j % SB) * STEP, t_o = tmem + C::O_COL + x * HD;
+#pragma unroll
+                    for (int kk = 0; kk < STEP / UMMA_K; ++kk)
+                        umma_ta(t_o, t_p + kk * 8, vd + (uint64_t)((kk * (UMMA_K * 128)) >> 4), id_o, (kk > 0 || j > 0) ? 1u : 0u);
+                    if (SB > 1 || j + 1 == n_x[u]) commit_at(b_o + x * 8);
+                    commit_at(b_ve + s * 8);
+                }
+                __syncwarp();
+                if (j + SB < n_x[u]) scores(x, j + SB);      // (behind P V in the tensor cores' order, which reads the same columns)
             }
         }
-        if (lane == 0) {                                     // tensor memory is given back only when nothing uses it any more
-            umma_commit(&drained[x]);
-            mbar_wait(&drained[x], 0);
+        if (elect_one()) {                                   // tensor memory is given back only when nothing uses it any more
+            commit_at(smem_u32(&drained[w]));
+            mbar_wait(&drained[w], 0);
         }
         __syncwarp();
-    } else if (warp < 8) {
+    } else {
         const int x = warp >> 2, r = (warp & 3) * 32 + lane, n_x = steps_of(x);
-        const int tok0 = row0 + (both ? 0 : x * TQ), toks = both ? n_tok : min(TQ, max(0, n_tok - x * TQ));
+        const int tok0 = row0 + (x & (R - 1)) * TQ, toks = min(TQ, max(0, n_tok - (x & (R - 1)) * TQ));
         const bool valid = r < toks * G;
         const bool warp_valid = (warp & 3) * 32 < toks * G;
         const int t = tok0 + (valid ? r / G : 0), head = kvh * G + r % G;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t t_s = tmem + lanes + C::S_COL + x * 128, t_o = tmem + lanes + C::O_COL + x * HD, t_p = tmem + lanes + C::P_COL + x * C::P_STRIDE;
-        {
+        const uint32_t t_o = tmem + lanes + C::O_COL + x * HD;
+        if (x < R) {
             const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)t * a.q_stride + (size_t)head * HD);
-            uint8_t* dst = q_s + x * C::BLOCK + r * 128;
+            uint8_t* dst = q_s + x * C::Q_BYTES + r * 128;
 #pragma unroll
             for (int c = 0; c < HD / 8; ++c)
                 *reinterpret_cast<uint4*>(dst + (c >> 3) * REGION + (((c & 7) ^ (r & 7)) << 4)) = valid ? src[c] : make_uint4(0u, 0u, 0u, 0u);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            arrive(&q_ready[x]);
+            arrive(smem_u32(&q_ready[x]));
         }
         const float sl2 = a.scale * LOG2E;                   // scores in units of log2(e)
         float m = -INFINITY;                                 // the max in use, scaled
         float2 l2 = make_float2(0.f, 0.f);
         bool ok = true;
-        auto wait = [&](uint64_t* bar, uint32_t parity, int code, int j) {
-            if (!mbar_wait(bar, parity)) { report(a.status, IMPARO_ST_WAIT_LIMIT, code, j, r); *gave_up = 1; ok = false; }
+        const uint32_t b_s = smem_u32(&s_ready[x * SB]), b_p = smem_u32(&p_ready[x]), b_o = smem_u32(&o_done[x]);
+        auto wait = [&](uint32_t bar, uint32_t parity, int code, int j) {
+            if (!wait_at(bar, parity)) { report(a.status, IMPARO_ST_WAIT_LIMIT, code, j, r); *gave_up = 1; ok = false; }
             ok = __all_sync(0xffffffffu, ok);
             fence_after();
         };
+        const int key_first = (first_step + at(x, 0)) * STEP, key_step = phases * STEP;
         for (int j = 0; j < n_x; ++j) {
-            wait(&s_ready[x], j & 1, 81, j);
+            const uint32_t t_s = tmem + lanes + (x * SB + j % SB) * STEP;
+            wait(b_s + j % SB * 8, (j / SB) & 1, 81, j);
             if (!ok) break;
-            uint32_t sv[128];
-            float corr = 1.f, m_new = m;
+            float sv[STEP];
+            float corr = 1.f;
             if (warp_valid) {
-                tmem_ld32(t_s, sv); tmem_ld32(t_s + 32, sv + 32); tmem_ld32(t_s + 64, sv + 64); tmem_ld32(t_s + 96, sv + 96);
+                uint32_t raw[STEP];
+                tmem_ld32(t_s, raw); tmem_ld32(t_s + 32, raw + 32);
                 wait_ld();
 #pragma unroll
-                for (int i = 0; i < 128; ++i) asm volatile("" : "+r"(sv[i]) :: "memory");
-            }
-            fence_before();
-            arrive(&s_free[x]);                              // the score columns may take the next step's product
-            bool rescale = false;
-            if (warp_valid) {
-                const int key0 = (first_step + at(x, j)) * STEP, lo = span.first - key0, hi = span.end - key0;
+                for (int i = 0; i < STEP; ++i) { asm volatile("" : "+r"(raw[i]) :: "memory"); sv[i] = __uint_as_float(raw[i]); }
+                const int key0 = key_first + j * key_step, lo = span.first - key0, hi = span.end - key0;
                 if (lo > 0 || hi < STEP) {
 #pragma unroll
-                    for (int i = 0; i < 128; ++i)
-                        if (i < lo || i >= hi) sv[i] = __float_as_uint(-INFINITY);
+                    for (int i = 0; i < STEP; ++i)
+                        if (i < lo || i >= hi) sv[i] = -INFINITY;
                 }
-                float mx0 = __uint_as_float(sv[0]), mx1 = __uint_as_float(sv[1]);
+                float mx[4];                                 // four running maxima: no long dependent chain
 #pragma unroll
-                for (int i = 2; i < 126; i += 4) {
-                    mx0 = max3(mx0, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
-                    mx1 = max3(mx1, __uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3]));
-                }
-                mx0 = fmaxf(max3(mx0, __uint_as_float(sv[126]), __uint_as_float(sv[127])), mx1) * sl2;     // (a rising function: scale > 0)
-                const bool grow = mx0 > m + GROW;            // (true for m = -inf and a finite max)
-                rescale = __any_sync(0xffffffffu, grow && j > 0);
-                m_new = grow ? mx0 : m;
+                for (int i = 0; i < 4; ++i) mx[i] = max3(sv[3 * i], sv[3 * i + 1], sv[3 * i + 2]);
+#pragma unroll
+                for (int i = 12; i < 60; i += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], sv[i + 2 * e], sv[i + 2 * e + 1]);
+                mx[0] = max3(max3(mx[0], sv[60], sv[61]), sv[62], sv[63]);
+                const float mx0 = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * sl2;         // (scale > 0: the max commutes with it)
+                // (true for m = -inf and a finite max, and for a max that is no number: a row with such a score has no result, nor
+                // has one with an infinite score)
+                const bool grow = !(mx0 <= m + GROW);
+                const float m_new = grow ? (mx0 == INFINITY ? __int_as_float(0x7fffffff) : mx0) : m;
                 corr = m == -INFINITY ? 0.f : ex2(m - m_new);
-            }
-            if (j > 0) wait(&o_done[x], (j - 1) & 1, 82, j);
-            if (!ok) break;
-            if (rescale) {                                   // the accumulated output of this warp's rows, in place
+                m = m_new;
+                if (__any_sync(0xffffffffu, grow && j > 0)) {                // the accumulated output of this warp's rows, in place
+                    // (one buffer of scores: these scores were made behind the P V of the step before)
+                    if (SB > 1) wait(b_o, (j - 1) & 1, 82, j);
+                    if (!ok) break;
 #pragma unroll 1
-                for (int c = 0; c < HD; c += 16) {
-                    float ov[16];
-                    tmem_ld16(t_o + c, ov);
-                    uint32_t ow[16];
+                    for (int c = 0; c < HD; c += 16) {
+                        float ov[16];
+                        tmem_ld16(t_o + c, ov);
+                        uint32_t ow[16];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) ow[e] = __float_as_uint(ov[e] * corr);
-                    tmem_st16(t_o + c, ow);
+                        for (int e = 0; e < 16; ++e) ow[e] = __float_as_uint(ov[e] * corr);
+                        tmem_st16(t_o + c, ow);
+                    }
+                    l2.x *= corr;
+                    l2.y *= corr;
                 }
             }
             if (warp_valid) {
-                l2.x *= corr; l2.y *= corr;
-                m = m_new;
                 const float nb = m == -INFINITY ? 0.f : -m;
                 const float2 sl = make_float2(sl2, sl2), base = make_float2(nb, nb);
+                float2 sum[2] = {l2, make_float2(0.f, 0.f)};
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {                // 32 keys = 16 columns of P
-                    uint32_t w[16];
+                for (int c = 0; c < 2; ++c) {                // 32 keys = 16 columns of P
+                    uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        float2 e = __ffma2_rn(make_float2(__uint_as_float(sv[c * 32 + 2 * i]), __uint_as_float(sv[c * 32 + 2 * i + 1])), sl, base);
-                        e.x = ex2(e.x);
-                        e.y = ex2(e.y);
-                        l2 = __fadd2_rn(l2, e);
-                        w[i] = pack_bf16(e.x, e.y);
+                        float2 e = __ffma2_rn(make_float2(sv[c * 32 + 2 * i], sv[c * 32 + 2 * i + 1]), sl, base);
+                        if (i * SP_FMA % 16 + SP_FMA >= 16) e = exp2_fma(e);
+                        else { e.x = ex2(e.x); e.y = ex2(e.y); }
+                        sum[i & 1] = __fadd2_rn(sum[i & 1], e);
+                        p[i] = pack_bf16(e.x, e.y);
                     }
-                    tmem_st16(t_p + c * 16, w);
-                    if (c == 1) { wait_st(); fence_before(); arrive(&p_half[x]); }
+                    tmem_st16(t_s + c * 16, p);
                 }
+                l2 = __fadd2_rn(sum[0], sum[1]);
                 wait_st();
-                fence_before();
-            } else {
-                arrive(&p_half[x]);
             }
-            arrive(&p_ready[x]);
+            // every phase is waited for, so that a wait by parity cannot take an earlier one for the one it means
+            if (SB > 1 && j > 0) {
+                wait(b_o, (j - 1) & 1, 84, j);
+                if (!ok) break;
+            }
+            fence_before();
+            arrive(b_p);
         }
-        if (ok && n_x > 0) wait(&o_done[x], (n_x - 1) & 1, 83, n_x);
+        if (ok && n_x > 0) wait(b_o, SB > 1 ? (n_x - 1) & 1 : 0, 83, n_x);
         float l = l2.x + l2.y;
         const size_t part = ((size_t)t * a.nh + head) * n_splits + chunk;
-        // the second half's results for the first one to add: [dim][row] and (max, sum) per row, where keys and values were
+        // the results of the tiles with the same rows, for the first of them to add: [tile][dims, max, sum][row], where keys and values were
         float* other = reinterpret_cast<float*>(k_s);
-        if (both) {
-            asm volatile("bar.sync 1, 256;" ::: "memory");   // both tiles' products have run
-            if (x == 1 && ok) {
+        constexpr int OTHER = (HD + 2) * TILE;
+        static_assert((size_t)(NT - 1) * OTHER * 4 <= (size_t)ST * 2 * C::KEY_BYTES, "the results of the other tiles");
+        if (phases > 1) {
+            asm volatile("bar.sync 1, %0;" ::"n"(NT * 128) : "memory");                      // all tiles' products have run
+            if (x >= R && ok) {
+                float* mine = other + (x - R) * OTHER + r;
                 if (n_x > 0 && warp_valid) {
 #pragma unroll 1
                     for (int c = 0; c < HD; c += 16) {
                         float o[16];
                         tmem_ld16(t_o + c, o);
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) other[(c + e) * TILE + r] = o[e];
+                        for (int e = 0; e < 16; ++e) mine[(c + e) * TILE] = o[e];
                     }
                 }
-                other[HD * TILE + r] = n_x > 0 ? m : -INFINITY;
-                other[(HD + 1) * TILE + r] = n_x > 0 ? l : 0.f;
+                mine[HD * TILE] = n_x > 0 ? m : -INFINITY;
+                mine[(HD + 1) * TILE] = n_x > 0 ? l : 0.f;
             }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            asm volatile("bar.sync 1, %0;" ::"n"(NT * 128) : "memory");
         }
-        if (ok && !__any_sync(0xffffffffu, *gave_up) && (x == 0 || !both) && warp_valid) {
-            float f = 1.f, g = 0.f, m_all = m;
-            if (both) {
-                const float m2 = other[HD * TILE + r], l_2 = other[(HD + 1) * TILE + r];
-                if (l_2 > 0.f) {
-                    m_all = fmaxf(m, m2);
-                    f = m == -INFINITY ? 0.f : ex2(m - m_all);
-                    g = ex2(m2 - m_all);
-                    l = l * f + l_2 * g;
+        if (ok && !__any_sync(0xffffffffu, *gave_up) && x < R && warp_valid) {
+            float m_all = m, f[NT];                          // the factor of each result
+#pragma unroll
+            for (int i = 1; i < NT; ++i)
+                if (i < phases && other[(x + (i - 1) * R) * OTHER + (HD + 1) * TILE + r] != 0.f)
+                    m_all = fmaxf(m_all, other[(x + (i - 1) * R) * OTHER + HD * TILE + r]);
+            f[0] = m == -INFINITY ? 0.f : ex2(m - m_all);
+            l *= f[0];
+#pragma unroll
+            for (int i = 1; i < NT; ++i) {
+                f[i] = 0.f;
+                if (i < phases) {
+                    const float* his = other + (x + (i - 1) * R) * OTHER + r;
+                    if (his[(HD + 1) * TILE] != 0.f) {
+                        f[i] = ex2(his[HD * TILE] - m_all);
+                        l += his[(HD + 1) * TILE] * f[i];
+                    }
                 }
             }
 #pragma unroll 1
             for (int c = 0; c < HD; c += 16) {
                 float o[16];
                 tmem_ld16(t_o + c, o);
-                if (g != 0.f) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] = o[e] * f + other[(c + e) * TILE + r] * g;
-                }
+                for (int e = 0; e < 16; ++e) o[e] *= f[0];
+#pragma unroll
+                for (int i = 1; i < NT; ++i)
+                    if (i < phases && f[i] != 0.f) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] += other[(x + (i - 1) * R) * OTHER + (c + e) * TILE + r] * f[i];
+                    }
                 if (valid) {
                     float4* dst = reinterpret_cast<float4*>(a.part_acc + part * HD + c);
 #pragma unroll
@@ -465,7 +552,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
     fence_before();
     __syncthreads();
-    if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    if (warp == C::MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 // ---- a row's own keys, and the join ----------------------------------------------------------------------------------
@@ -630,50 +717,74 @@ own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __rest
         live = min(a.n_shared, (steps + per_chunk - 1) / per_chunk);
     }
     if (JOIN) pdl_wait();                                    // the kernel that makes the partial results is complete
-    for (int i = tid; i < n_heads * (HD / 4); i += OWN_WARPS * 32) {
-        const int h = i / (HD / 4), d = i % (HD / 4) * 4;
+    // a warp a head: the lanes are the partial results (their largest score and sum) first, then the dims
+    constexpr int PER = HD / 32;
+    for (int h = warp; h < n_heads; h += OWN_WARPS) {
         const size_t row = (size_t)t * a.nh + head0 + h;
-        const float* ml = a.part_ml + row * n_splits * 2;
-        float m = -INFINITY;
-        for (int w = 0; w < OWN_WARPS; ++w) m = fmaxf(m, w_m[w][h]);
-        if (JOIN) {
-            for (int s = 0; s < live; ++s) if (__ldcg(ml + 2 * s + 1) != 0.f) m = fmaxf(m, __ldcg(ml + 2 * s) * LOG2E);
-            if (sinks) m = fmaxf(m, sinks[head0 + h] * LOG2E);
-        }
-        float l = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float m = lane < OWN_WARPS ? w_m[lane][h] : -INFINITY, l = 0.f, acc[PER];
+        m = warp_max(m);
+        const float own_f = lane < OWN_WARPS && w_l[lane][h] != 0.f ? ex2(w_m[lane][h] - m) : 0.f;
+        l = warp_sum(lane < OWN_WARPS ? w_l[lane][h] * own_f : 0.f);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+#pragma unroll
         for (int w = 0; w < OWN_WARPS; ++w) {
-            if (w_l[w][h] == 0.f) continue;
-            const float f = ex2(w_m[w][h] - m);
-            const float4 x = *reinterpret_cast<const float4*>(&w_o[w][h][d]);
-            l += w_l[w][h] * f;
-            acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
+            const float f = __shfl_sync(0xffffffffu, own_f, w);
+            if (f != 0.f) {
+#pragma unroll
+                for (int e = 0; e < PER; ++e) acc[e] += w_o[w][h][lane * PER + e] * f;
+            }
         }
         if (JOIN) {
-            const float4* part = reinterpret_cast<const float4*>(a.part_acc + row * n_splits * HD + d);
-#pragma unroll 4
-            for (int s = 0; s < live; ++s) {
-                const float4 x = __ldcg(part + (size_t)s * (HD / 4));
-                const float ls = __ldcg(ml + 2 * s + 1);
-                if (ls != 0.f) {
-                    const float f = ex2(__ldcg(ml + 2 * s) * LOG2E - m);
-                    l += ls * f;
-                    acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
+            const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row * n_splits;
+            const float* part = a.part_acc + row * n_splits * HD + lane * PER;
+            for (int s0 = 0; s0 < live; s0 += 32) {
+                const float2 v = s0 + lane < live ? __ldcg(ml + s0 + lane) : make_float2(-INFINITY, 0.f);
+                const float m_new = fmaxf(m, warp_max(v.y != 0.f ? v.x * LOG2E : -INFINITY));
+                const float f = v.y != 0.f ? ex2(v.x * LOG2E - m_new) : 0.f;
+                const float corr = m == -INFINITY ? 0.f : ex2(m - m_new);
+                m = m_new;
+                l = l * corr + warp_sum(v.y * f);
+#pragma unroll
+                for (int e = 0; e < PER; ++e) acc[e] *= corr;
+                const int n = min(32, live - s0);
+                for (int s = 0; s < n; s += 8) {
+                    float x[8][PER];                         // eight partial results on their way at once
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+#pragma unroll
+                        for (int e = 0; e < PER; ++e) x[u][e] = s + u < n ? __ldcg(part + (size_t)(s0 + s + u) * HD + e) : 0.f;
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        const float fs = __shfl_sync(0xffffffffu, f, (s + u) & 31);
+                        if (s + u < n && fs != 0.f) {        // (a result of sum 0 has no values)
+#pragma unroll
+                            for (int e = 0; e < PER; ++e) acc[e] += x[u][e] * fs;
+                        }
+                    }
                 }
             }
-            if (sinks) l += ex2(sinks[head0 + h] * LOG2E - m);
-            const float inv = l > 0.f ? 1.0f / l : 0.f;
-            *reinterpret_cast<uint2*>(out + row * HD + d) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+            if (sinks) {
+                const float sink = sinks[head0 + h] * LOG2E, m_new = fmaxf(m, sink), corr = m == -INFINITY ? 0.f : ex2(m - m_new);
+                l = l * corr + ex2(sink - m_new);
+#pragma unroll
+                for (int e = 0; e < PER; ++e) acc[e] *= corr;
+            }
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+            for (int e = 0; e < PER; e += 2)
+                *reinterpret_cast<uint32_t*>(out + row * HD + lane * PER + e) = pack_bf16(acc[e] * inv, acc[e + 1] * inv);
         } else {
-            *reinterpret_cast<float4*>(a.part_acc + (row * n_splits + a.n_shared + split) * HD + d) = acc;
-            if (d == 0) {
-                float* mine = a.part_ml + (row * n_splits + a.n_shared + split) * 2;
-                mine[0] = m == -INFINITY ? -INFINITY : m * LN2;
-                mine[1] = l;
+            const size_t mine = row * n_splits + a.n_shared + split;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) a.part_acc[mine * HD + lane * PER + e] = acc[e];
+            if (lane == 0) {
+                a.part_ml[mine * 2] = m == -INFINITY ? -INFINITY : m * LN2;
+                a.part_ml[mine * 2 + 1] = l;
             }
             // a row of no group has no part in the shared stretches
-            if (d == 0 && split == 0 && group < 0)
-                for (int s = 0; s < a.n_shared; ++s) {
+            if (split == 0 && group < 0)
+                for (int s = lane; s < a.n_shared; s += 32) {
                     a.part_ml[(row * n_splits + s) * 2] = -INFINITY;
                     a.part_ml[(row * n_splits + s) * 2 + 1] = 0.f;
                 }
@@ -718,8 +829,9 @@ static int launch_hd(const Args& a, __nv_bfloat16* out, const float* sinks, cuda
         if (device >= 0 && device < 64) configured[device] = true;
     }
     const int n_splits = a.n_own == 1 ? a.n_shared : a.n_shared + a.n_own;
-    const long long units = (a.n_rows + 2 * TQ - 1) / (2 * TQ) + a.n_groups - 1;       // every group may end a tile early
-    e = launch(shared_tc_kernel<HD>, dim3(a.nkv, a.n_shared, (unsigned)units), dim3(TC_THREADS), Shape<HD>::SMEM, stream, mk, mv, a, n_splits);
+    const int tokens = Shape<HD>::TILES * TQ;
+    const long long units = (a.n_rows + tokens - 1) / tokens + a.n_groups - 1;       // every group may end a tile early
+    e = launch(shared_tc_kernel<HD>, dim3(a.nkv, a.n_shared, (unsigned)units), dim3(Shape<HD>::THREADS), Shape<HD>::SMEM, stream, mk, mv, a, n_splits);
     if (e != cudaSuccess) return (int)e;
     const dim3 grid(a.nkv * head_tiles, a.n_rows, a.n_own);
     e = a.n_own == 1 ? launch(own_tc_kernel<HD, true>, grid, dim3(OWN_WARPS * 32), 0, stream, a, out, sinks, n_splits)
@@ -731,7 +843,7 @@ int launch_tc(const Args& a, void* out, const float* sinks, cudaStream_t stream)
     const int G = a.nh / a.nkv;
     if ((a.hd != 64 && a.hd != 128) || G > TILE || !(a.scale > 0.f)) return -8;
     if (a.page_size != 16 && a.page_size != 32 && a.page_size != 64 && a.page_size % STEP != 0) return -8;
-    if (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)out | (uintptr_t)a.part_acc) & 15) return -8;
+    if (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)out | (uintptr_t)a.part_acc | (uintptr_t)a.part_ml) & 15) return -8;
     if (a.q_stride % 8 != 0 || a.chunk_shared % STEP != 0) return -8;
     if (a.n_rows > 65535 || a.n_own > 65535 || a.n_rows + a.n_groups > 65535) return -8;
     return a.hd == 64 ? launch_hd<64>(a, (__nv_bfloat16*)out, sinks, stream) : launch_hd<128>(a, (__nv_bfloat16*)out, sinks, stream);

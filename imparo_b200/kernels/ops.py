@@ -1657,18 +1657,19 @@ def shared_prefix_plan(n_rows: int, n_groups: int, nh: int, nkv: int, hd: int, d
     sms = sms if sms is not None else sm_count()
     group = nh // nkv
     if dtype == torch.bfloat16 and hd in (64, 128) and group <= 128:
-        # A CTA per SM takes up to two tiles of 128 rows through a stretch of 128-key steps; rows that fill one tile are taken by both,
-        # a step each.  The number of stretches is the one with the least time: rounds of CTAs, each as long as its steps and five
-        # more (what a CTA's start and end cost), and the partial results, written and read (in steps of 0.7 us at 6.5 TB/s).
-        tokens = 128 // group
+        # A CTA per SM takes up to four (head size 64) or two tiles of 128 rows through a stretch of 64-key steps; rows that fill fewer
+        # tiles are given to all of them, a step each.  The number of stretches is the one with the least time: rounds of CTAs, each as
+        # long as its steps (a tile's exponentials, or the step's keys and values from memory) and what a CTA's start and end cost,
+        # and the partial results, written and read.  In units of a tile's step, about 0.2 us.
+        tokens, tiles = 128 // group, 4 if hd == 64 else 2
         each = -(-n_rows // n_groups)
-        ctas = nkv * n_groups * -(-each // (2 * tokens))
-        steps = max(1, -(-most_shared // 128))
-        per_step = 2 if each <= tokens else 1
-        cost = lambda n: -(-ctas * n // sms) * (-(-(-(-steps // n)) // per_step) + 5) + n * n_rows * nh * hd * 1.8e-6
+        ctas = nkv * n_groups * -(-each // (tiles * tokens))
+        steps = max(1, -(-most_shared // 64))
+        per_step = max(min(tiles, -(-each // tokens)), 2 * hd / 64)
+        cost = lambda n: -(-ctas * n // sms) * (-(-steps // n) * per_step + 25) + n * n_rows * nh * hd * 6e-6
         n_shared = min(range(1, min(steps, 2 * sms) + 1), key=cost)
-        chunk_shared = -(-steps // n_shared) * 128
-        n_shared = -(-steps * 128 // chunk_shared)
+        chunk_shared = -(-steps // n_shared) * 64
+        n_shared = -(-steps * 64 // chunk_shared)
         # one stretch of own keys is joined with the shared ones at once; more only where few rows have long ones
         n_own = max(1, min(-(-most_own // 512), -(-2 * sms // (n_rows * nkv * -(-group // 16))), 256))
         chunk_own = max(64, -(-(-(-most_own // n_own)) // 64) * 64)
