@@ -46,19 +46,15 @@ struct Args {
 };
 
 struct Shared {
-    union {
-        struct { uint32_t n[BINS], lo[BINS], hi[BINS]; } own;      // this CTA's histogram: counts, weights in two halves
-        u64 list[LIST];                                            // entries of one bin, the same in every CTA of the cluster
-    };
-    uint32_t all_n[BINS];                                          // the cluster's histogram
-    u64 all_w[BINS];
+    uint32_t n[BINS], lo[BINS], hi[BINS];                          // this CTA's histogram: counts, weights in two halves
+    u64 list[LIST];                                                // entries that are sorted
     double table[64];                                              // 2^(i / 64)
     u64 warp_w[WARPS + 1];
     uint32_t warp_n[WARPS + 1];
     u64 part_top, part_w;                                          // read by the other CTAs
-    uint32_t part_n, list_n;
-    u64 before_w, found_cut;
-    uint32_t before_n, bin, found;
+    uint32_t part_n, list_n, gathered;
+    u64 before_w, found_cut, total_w;
+    uint32_t before_n, bin, found, total_n;
 };
 
 // a logit as a whole number of the same order, and back; equal logits have equal numbers (the zero's sign is dropped on loading)
@@ -116,6 +112,9 @@ __device__ __forceinline__ u64 part_of(float x, u64 num, bool up) {
     }
     return q + (up && rest != 0 ? 1 : 0);
 }
+
+// The weight that the running sum has to pass for the pick.  (The largest entry always stays: total >= 1.)
+__device__ __forceinline__ u64 target_of(float u, u64 total) { return u < 1.f ? (u > 0.f ? part_of(u, total, false) : 0) : total - 1; }
 
 template <typename T>
 __device__ __forceinline__ float load1(const T* p) { return clean(to_f32(*p)); }
@@ -179,6 +178,7 @@ sample_filtered_kernel(const Args a) {
     auto value = [&](int i) -> float { return STAGED ? staged[i] : load1(row + i); };
 
     if (tid < 64) s.table[tid] = exp2((double)tid / 64.0);
+    if (tid == 0) s.gathered = 0;
 
     // ---- the stretch into shared memory, its first largest entry ----
     u64 top = 0;                                                   // (0: no number above minus infinity)
@@ -236,48 +236,102 @@ sample_filtered_kernel(const Args a) {
     // the bin of a logit: never falls as the logit falls, whatever the rounding
     auto bin_of = [&](float v) -> int { return v == topf ? 0 : min(BINS - 1, (int)((topf - v) * per_bin)); };
 
-    // A histogram over the entries that `take` maps to a bin (-1: none), summed over the cluster into all_n (and all_w).
-    auto histogram = [&](bool weights, auto take) {
-        __syncthreads();
-        for (int i = tid; i < BINS; i += THREADS) { s.own.n[i] = 0; s.own.lo[i] = 0; s.own.hi[i] = 0; }
+    // The cluster's histogram over the entries that `take` maps to a bin (-1: none): a thread gets its two bins' sums.
+    bool first_histogram = true;
+    auto histogram = [&](bool weights, auto take, uint32_t (&n)[2], u64 (&w)[2]) {
+        if (!first_histogram) cluster.sync();                      // the others have read the one before
+        first_histogram = false;
+        for (int i = tid; i < BINS; i += THREADS) { s.n[i] = 0; s.lo[i] = 0; s.hi[i] = 0; }
         __syncthreads();
         for (int i = tid; i < count; i += THREADS) {
             const float v = value(i);
             const int b = take(v, lo + i);
             if (b >= 0) {
-                atomicAdd(&s.own.n[b], 1u);
+                atomicAdd(&s.n[b], 1u);
                 if (weights) {
-                    const u64 w = weight(v);
-                    const uint32_t low = (uint32_t)w, old = atomicAdd(&s.own.lo[b], low);
-                    const uint32_t high = (uint32_t)(w >> 32) + (old + low < old ? 1u : 0u);
-                    if (high) atomicAdd(&s.own.hi[b], high);
+                    const u64 x = weight(v);
+                    const uint32_t low = (uint32_t)x, old = atomicAdd(&s.lo[b], low);
+                    const uint32_t high = (uint32_t)(x >> 32) + (old + low < old ? 1u : 0u);
+                    if (high) atomicAdd(&s.hi[b], high);
                 }
             }
         }
         cluster.sync();
-        const int share = BINS / ranks;                            // ranks is a power of two
-        for (int i = rank * share + tid; i < (rank + 1) * share; i += THREADS) {
-            uint32_t n = 0;
-            u64 w = 0;
-            for (int k = 0; k < ranks; ++k) {
-                const Shared* other = cluster.map_shared_rank(&s, k);
-                n += other->own.n[i];
-                if (weights) w += ((u64)other->own.hi[i] << 32) + other->own.lo[i];
-            }
-            for (int k = 0; k < ranks; ++k) {
-                Shared* other = cluster.map_shared_rank(&s, k);
-                other->all_n[i] = n;
-                other->all_w[i] = w;
+        n[0] = n[1] = 0;
+        w[0] = w[1] = 0;
+        for (int k = 0; k < ranks; ++k) {
+            const Shared* other = cluster.map_shared_rank(&s, k);
+            const uint2 x = *reinterpret_cast<const uint2*>(&other->n[2 * tid]);
+            n[0] += x.x;
+            n[1] += x.y;
+            if (weights) {
+                const uint2 low = *reinterpret_cast<const uint2*>(&other->lo[2 * tid]), high = *reinterpret_cast<const uint2*>(&other->hi[2 * tid]);
+                w[0] += ((u64)high.x << 32) + low.x;
+                w[1] += ((u64)high.y << 32) + low.y;
             }
         }
-        cluster.sync();
+    };
+    auto kept_bound = [&]() -> u64 {                               // min_p as a bound on the logit: w >= min_p
+        if (!a.min_p || !(a.min_p[r] > 0.f)) return 1;             // (1: every number above minus infinity)
+        const float p = a.min_p[r];
+        if (p > 1.f) return top;                                   // only the first largest entry stays
+        const float bound = __double2float_ru((double)topf + (double)temp * log((double)p));
+        return bound > -INFINITY ? (u64)ordered(bound + 0.0f) << 32 : 1;
+    };
+    const int top_k = a.top_k && a.top_k[r] > 0 && a.top_k[r] < a.vocab ? a.top_k[r] : 0;          // 0: all
+    const float top_p = a.top_p && a.top_p[r] < 1.f ? fmaxf(a.top_p[r], 0.f) : 1.f;                // 1: all
+
+    // All that is left to do, by the first CTA alone, where the list holds a beginning of the order that reaches beyond every cut:
+    // sorts it, cuts it, and picks from what stays in the order of the vocabulary.  need: the weight before which entries stay, 0:
+    // top_p of the first top_k's weight, which the list holds.
+    auto finish = [&](int size, u64 need) {
+        int pow2 = 64;
+        while (pow2 < size) pow2 <<= 1;
+        for (int i = size + tid; i < pow2; i += THREADS) s.list[i] = 0;
+        sort_list(s.list, pow2);
+        const int stay_k = top_k > 0 ? min(size, top_k) : size, i0 = 2 * tid;
+        const u64 e[2] = {i0 < stay_k ? s.list[i0] : 0, i0 + 1 < stay_k ? s.list[i0 + 1] : 0};
+        u64 x[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) x[i] = e[i] ? weight(unordered((uint32_t)(e[i] >> 32))) : 0;
+        uint32_t bn;
+        u64 bw;
+        block_before(s, 0, x[0] + x[1], bn, bw);
+        if (tid == THREADS - 1) s.total_w = bw + x[0] + x[1];
+        if (tid == 0) s.found = 0;
+        __syncthreads();
+        if (need == 0) need = top_p < 1.f ? max(part_of(top_p, s.total_w, true), 1ull) : ~0ull;
+        const u64 bound = kept_bound();
+        if (e[0] && bw < need && e[0] >= bound) atomicMax(&s.found, (uint32_t)i0 + 1);
+        if (e[1] && bw + x[0] < need && e[1] >= bound) atomicMax(&s.found, (uint32_t)i0 + 2);
+        __syncthreads();
+        const int stay = max(1, (int)s.found);                     // (the first entry always stays)
+        // by index: the larger key is the smaller index, with the logit behind it
+        for (int i = 0; i < 2; ++i) s.list[i0 + i] = i0 + i < stay ? (e[i] << 32) | (e[i] >> 32) : 0;
+        pow2 = 2;
+        while (pow2 < stay) pow2 <<= 1;
+        sort_list(s.list, pow2);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) x[i] = i0 + i < stay ? weight(unordered((uint32_t)s.list[i0 + i])) : 0;
+        block_before(s, 0, x[0] + x[1], bn, bw);
+        if (tid == THREADS - 1) s.total_w = bw + x[0] + x[1];
+        __syncthreads();
+        const u64 target = target_of(a.uniform[r], s.total_w);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (bw <= target && target < bw + x[i]) {
+                a.out[r] = (int)~(uint32_t)(s.list[i0 + i] >> 32);
+                if (a.kept) a.kept[r] = stay;
+            }
+            bw += x[i];
+        }
     };
 
-    // The cut behind the last entry kept: entries are counted (by_rank: the first `need` of the order stay) or weighed (those stay
-    // before which less than `need` weighs), over the entries at or above `least`.  whole_w: the weight of all of these.
-    auto find_cut = [&](bool by_rank, u64 least, float share_of_total) -> u64 {
-        u64 need = 0;
-        if (by_rank) need = (u64)a.top_k[r];
+    // The cut behind the last entry kept: entries are counted (by_rank: the first top_k of the order stay) or weighed (those stay before
+    // which less than top_p of the total weighs), over the entries at or above `least`.  Returns 0 where the first CTA has finished
+    // the row: the beginning of the order up to the cut's bin fits the list.
+    auto find_cut = [&](bool by_rank, u64 least) -> u64 {
+        u64 need = by_rank ? (u64)top_k : 0;
         uint32_t before_n = 0;
         u64 before_w = 0;
         int chosen_bin = -1;                                       // the bin of equal width, then the prefix of the ordered logit
@@ -285,6 +339,8 @@ sample_filtered_kernel(const Args a) {
         for (int level = 0; ; ++level) {
             // level 0: bins of equal width; levels 1 to 4: the next 10, 10, 10 and 2 bits of the ordered logit
             const int down = level == 0 ? 32 : level < 4 ? 32 - 10 * level : 0, up = level == 1 ? 0 : 42 - 10 * level;
+            uint32_t hn[2];
+            u64 hw[2];
             histogram(!by_rank, [&](float v, int index) -> int {
                 if (!(v > -INFINITY) || entry(v, index) < least) return -1;
                 const int b = bin_of(v);
@@ -292,34 +348,47 @@ sample_filtered_kernel(const Args a) {
                 const uint32_t k = ordered(v);
                 if (b != chosen_bin || (level > 1 && (k >> (level == 4 ? 2 : up)) != prefix)) return -1;
                 return BINS - 1 - (int)((k >> down) & (level == 4 ? 3u : 1023u));
-            });
-            const uint32_t n0 = s.all_n[2 * tid], n1 = s.all_n[2 * tid + 1];
-            const u64 w0 = s.all_w[2 * tid], w1 = s.all_w[2 * tid + 1];
+            }, hn, hw);
             uint32_t bn;
             u64 bw;
-            block_before(s, n0 + n1, w0 + w1, bn, bw);
+            block_before(s, hn[0] + hn[1], hw[0] + hw[1], bn, bw);
             if (level == 0) {
-                if (tid == THREADS - 1) { s.before_n = bn + n0 + n1; s.before_w = bw + w0 + w1; }
+                if (tid == THREADS - 1) { s.total_n = bn + hn[0] + hn[1]; s.total_w = bw + hw[0] + hw[1]; }
                 __syncthreads();
                 if (by_rank) {
-                    if (need >= s.before_n) return least;          // there are no more than top_k
+                    if (need >= s.total_n) return least;           // there are no more than top_k
                 } else {
-                    need = part_of(share_of_total, s.before_w, true);
-                    if (need == 0) need = 1;                       // the first entry always stays
+                    need = max(part_of(top_p, s.total_w, true), 1ull);               // (the first entry always stays)
                 }
-                __syncthreads();
             }
             // the first bin at whose end the count or the weight has been reached
             bn += before_n;
             bw += before_w;
-            const u64 at = by_rank ? bn : bw, x0 = by_rank ? n0 : w0, x1 = by_rank ? n1 : w1;
-            if (at < need && at + x0 >= need) { s.bin = 2 * tid; s.before_n = bn; s.before_w = bw; s.found = n0; }
-            else if (at + x0 < need && at + x0 + x1 >= need) { s.bin = 2 * tid + 1; s.before_n = bn + n0; s.before_w = bw + w0; s.found = n1; }
+            const u64 at = by_rank ? bn : bw, x0 = by_rank ? hn[0] : hw[0], x1 = by_rank ? hn[1] : hw[1];
+            if (at < need && at + x0 >= need) { s.bin = 2 * tid; s.before_n = bn; s.before_w = bw; s.found = hn[0]; }
+            else if (at + x0 < need && at + x0 + x1 >= need) { s.bin = 2 * tid + 1; s.before_n = bn + hn[0]; s.before_w = bw + hw[0]; s.found = hn[1]; }
             __syncthreads();
             before_n = s.before_n;
             before_w = s.before_w;
             const int bin = (int)s.bin;
             const uint32_t found = s.found;
+            if (level == 0 && before_n + found <= LIST) {
+                Shared* first = cluster.map_shared_rank(&s, 0);
+                for (int i = tid; i - lane < count; i += THREADS) {
+                    const float v = i < count ? value(i) : -INFINITY;
+                    const bool in = v > -INFINITY && bin_of(v) <= bin && entry(v, lo + i) >= least;
+                    const unsigned mask = __ballot_sync(0xffffffffu, in);
+                    if (mask) {
+                        uint32_t place = 0;
+                        if (lane == __ffs(mask) - 1) place = atomicAdd(&first->gathered, (uint32_t)__popc(mask));
+                        place = __shfl_sync(0xffffffffu, place, __ffs(mask) - 1) + __popc(mask & ((1u << lane) - 1u));
+                        if (in) first->list[place] = entry(v, lo + i);
+                    }
+                }
+                cluster.sync();
+                if (rank == 0) finish((int)(before_n + found), by_rank ? 0 : need);
+                return 0;
+            }
             if (level == 0) chosen_bin = bin;
             else prefix = level == 4 ? prefix : (level == 1 ? 0u : prefix << 10) | (uint32_t)(BINS - 1 - bin);
             const uint32_t last_digit = level == 4 ? (uint32_t)(BINS - 1 - bin) : 0u;
@@ -331,9 +400,8 @@ sample_filtered_kernel(const Args a) {
             };
             if (found <= LIST) {
                 // the bin's entries to every CTA of the cluster, sorted there
-                uint32_t mine = s.own.n[bin], first = 0;
-                for (int k = 0; k < rank; ++k) first += cluster.map_shared_rank(&s, k)->own.n[bin];
-                cluster.sync();                                    // the histograms are read: the list takes their place
+                uint32_t mine = s.n[bin], first = 0;
+                for (int k = 0; k < rank; ++k) first += cluster.map_shared_rank(&s, k)->n[bin];
                 if (tid == 0) s.list_n = first;
                 int size = 32;
                 while (size < (int)found) size <<= 1;
@@ -405,17 +473,9 @@ sample_filtered_kernel(const Args a) {
     };
 
     u64 cut = 1;                                                   // every number above minus infinity
-    if (a.top_k && a.top_k[r] > 0 && a.top_k[r] < a.vocab) cut = find_cut(true, cut, 0.f);
-    if (a.top_p && a.top_p[r] < 1.f) cut = find_cut(false, cut, a.top_p[r] > 0.f ? a.top_p[r] : 0.f);
-    if (a.min_p && a.min_p[r] > 0.f) {
-        // w >= min_p as a bound on the logit; above 1 only the first largest entry stays
-        const float p = a.min_p[r];
-        if (p > 1.f) cut = top;
-        else {
-            const float bound = __double2float_ru((double)topf + (double)temp * log((double)p));
-            if (bound > -INFINITY) cut = max(cut, (u64)ordered(bound + 0.0f) << 32);
-        }
-    }
+    if (top_k > 0 && (cut = find_cut(true, cut)) == 0) return;
+    if (top_p < 1.f && (cut = find_cut(false, cut)) == 0) return;
+    cut = max(cut, kept_bound());
 
     // ---- the kept weights in vocabulary order: warps own contiguous stretches, whose sums are whole numbers ----
     const int seg = ((count + WARPS - 1) / WARPS + 31) / 32 * 32;
@@ -451,8 +511,7 @@ sample_filtered_kernel(const Args a) {
         kept += other->part_n;
     }
     for (int i = 0; i < warp; ++i) before += s.warp_w[i];
-    const float u = a.uniform[r];
-    const u64 target = u < 1.f ? (u > 0.f ? part_of(u, whole, false) : 0) : whole - 1;       // the largest entry weighs: whole >= 1
+    const u64 target = target_of(a.uniform[r], whole);
     if (before <= target && target < before + w) {                 // (warp-uniform) this warp holds the pick
         for (int i = s0 + lane; i - lane < s1; i += 32) {
             u64 x = 0;

@@ -1561,11 +1561,25 @@ def sample_rows(logits, temperature, uniform, out) -> None:
                                              logits.stride(0), _stream()), "sample_rows")
 
 
-def _here(what: str, *ts) -> None:
-    """All on the current device, whose stream the launch goes to."""
-    current = torch.cuda.current_device()
+def _placed(what: str, *ts) -> None:
+    """All dense and on the current device, whose stream the launch goes to (None: not given)."""
+    here = -1
     for t in ts:
-        _need(t is None or t.device.index == current, f"{what}: a tensor is on another device than the current one")
+        if t is None:
+            continue
+        if not t.is_cuda or not t.is_contiguous():
+            _cuda(t)
+        if here < 0:
+            here = _current_device() if _current_device is not None else torch.cuda.current_device()
+        if t.get_device() != here:
+            raise KernelError(f"{what}: a tensor is on another device than the current one")
+
+
+def _typed(what: str, dtype: torch.dtype, *named) -> None:
+    """(tensor or None, fewest entries, name) each: of this type and as long."""
+    for t, count, name in named:
+        if t is not None and (t.dtype != dtype or t.numel() < count):
+            raise KernelError(f"{what}: {name} must be {dtype} with {count} entries at least")
 
 
 def sample_filtered(logits, temperature, uniform, out, top_k=None, top_p=None, min_p=None, kept=None) -> None:
@@ -1581,18 +1595,16 @@ def sample_filtered(logits, temperature, uniform, out, top_k=None, top_p=None, m
     temperature <= 0: the first maximum.  NaN counts as minus infinity, which is never picked; a row of nothing else gives 0.
     kept (int32 or None): how many tokens the filters left (1 where greedy, 0 in a row of nothing).
     temperature and uniform float32, out int32, all one value per row."""
-    _need(logits.is_cuda and logits.dim() == 2, "sample_filtered: logits [rows, vocab] on a CUDA device")
-    _cuda(temperature, uniform, out, top_k, top_p, min_p, kept)
-    _here("sample_filtered", logits, temperature, uniform, out, top_k, top_p, min_p, kept)
+    if not logits.is_cuda or logits.dim() != 2 or temperature is None or uniform is None:
+        raise KernelError("sample_filtered: logits [rows, vocab] on a CUDA device, temperature and uniform are needed")
+    _placed("sample_filtered", temperature, uniform, out, top_k, top_p, min_p, kept)
     n, vocab = logits.shape
     code = _code(logits)
+    _need(logits.get_device() == out.get_device(), "sample_filtered: a tensor is on another device than the current one")
     _need(1 <= vocab <= 1 << 24 and n <= 1 << 20, "sample_filtered: 1 to 2^24 entries per row, at most 2^20 rows")
     _need((vocab == 1 or logits.stride(1) == 1) and (n < 2 or logits.stride(0) >= vocab), "sample_filtered: a row's logits must lie side by side")
-    _need(temperature is not None and uniform is not None, "sample_filtered: temperature and uniform are needed")
-    for t, dtype, name in ((temperature, torch.float32, "temperature"), (uniform, torch.float32, "uniform"), (out, torch.int32, "out"),
-                           (top_k, torch.int32, "top_k"), (top_p, torch.float32, "top_p"), (min_p, torch.float32, "min_p"),
-                           (kept, torch.int32, "kept")):
-        _need(t is None or (t.dtype == dtype and t.numel() >= n), f"sample_filtered: {name} must be {dtype}, one value per row")
+    _typed("sample_filtered", torch.float32, (temperature, n, "temperature"), (uniform, n, "uniform"), (top_p, n, "top_p"), (min_p, n, "min_p"))
+    _typed("sample_filtered", torch.int32, (out, n, "out"), (top_k, n, "top_k"), (kept, n, "kept"))
     if n == 0:
         return
     _check(_lib.kernels().imparo_sample_filtered(_ptr(logits), code, logits.stride(0) if n > 1 else vocab, _ptr(temperature), _ptr(uniform),
@@ -1614,28 +1626,26 @@ def step_tables(lengths, counts, free_pages, held, page_size, n_pages, table, po
     taken (int32 [1]): how many of the free pages are now in use.
 
     A free list that is too short, a table or token arrays that are too narrow, negative lengths and pages outside [0, n_pages) are
-    recorded in the status word (read_status raises); nothing is written out of range, what has no page gets -1."""
-    _cuda(lengths, counts, free_pages, held, table, positions, item_of_token, row_start, slots, taken, status, parent, shared)
-    _here("step_tables", lengths, counts, free_pages, held, table, positions, item_of_token, row_start, slots, taken, status, parent, shared)
-    _need(held.dim() == 2 and table.dim() == 2 and held.shape[0] == table.shape[0], "step_tables: held and table must be [items, blocks]")
+    recorded in the status word (read_status raises); nothing is written out of range, what has no page gets -1.  What is written must
+    not overlap what is read."""
+    _placed("step_tables", lengths, counts, free_pages, held, table, positions, item_of_token, row_start, slots, taken, status, parent, shared)
+    _need(held.dim() == 2 and table.dim() == 2, "step_tables: held and table must be [items, blocks]")
     n, width = table.shape
-    for t, count, name in ((lengths, n, "lengths"), (counts, n, "counts"), (row_start, n + 1, "row_start"), (taken, 1, "taken"),
-                           (parent, n, "parent"), (shared, n, "shared"), (free_pages, 0, "free_pages"), (held, 0, "held"), (table, 0, "table"),
-                           (positions, 0, "positions"), (item_of_token, positions.numel(), "item_of_token"), (status, 4, "status")):
-        _need(t is None or (t.dtype == torch.int32 and t.numel() >= count), f"step_tables: {name} must be int32 with {count} entries at least")
-    _need(slots.dtype == torch.int64 and slots.numel() >= positions.numel(), "step_tables: slots must be int64, one per position")
+    held_items, held_width = held.shape
+    tokens, n_free = positions.numel(), free_pages.numel()
+    _typed("step_tables", torch.int32, (lengths, n, "lengths"), (counts, n, "counts"), (row_start, n + 1, "row_start"), (taken, 1, "taken"),
+           (parent, n, "parent"), (shared, n, "shared"), (free_pages, 0, "free_pages"), (held, 0, "held"), (table, 0, "table"),
+           (positions, 0, "positions"), (item_of_token, tokens, "item_of_token"), (status, 4, "status"))
+    _typed("step_tables", torch.int64, (slots, tokens, "slots"))
     _need((parent is None) == (shared is None), "step_tables: parent and shared go together")
-    _need(1 <= n <= 1 << 24 and width >= 1 and page_size >= 1 and n_pages >= 1, "step_tables: items, blocks, page size and pages")
+    _need(held_items == n and 1 <= n <= 1 << 24 and width >= 1 and page_size >= 1 and n_pages >= 1, "step_tables: items, blocks, page size and pages")
     _need(n_pages * page_size <= 1 << 40, "step_tables: slots of at most 2^40")
-    written = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (table, positions, item_of_token, row_start, slots, taken)]
-    for t in (held, free_pages, lengths, counts, parent, shared):
-        if t is not None and t.numel():
-            lo, hi = t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
-            _need(all(hi <= a or b <= lo for a, b in written), "step_tables: what is read and what is written must not overlap")
-    _check(_lib.kernels().imparo_step_tables(_ptr(lengths), _ptr(counts), _ptr(free_pages), free_pages.numel(), _ptr(held), held.shape[1],
-                                             _ptr(parent), _ptr(shared), n, int(page_size), int(n_pages), _ptr(table), width,
-                                             _ptr(positions), _ptr(item_of_token), positions.numel(), _ptr(row_start), _ptr(slots),
-                                             _ptr(taken), _ptr(status), _stream()), "step_tables")
+    at_table, at_held = table.data_ptr(), held.data_ptr()
+    _need(at_table >= at_held + 4 * n * held_width or at_held >= at_table + 4 * n * width, "step_tables: held and table must not overlap")
+    _check(_lib.kernels().imparo_step_tables(lengths.data_ptr(), counts.data_ptr(), free_pages.data_ptr(), n_free, at_held, held_width,
+                                             _ptr(parent), _ptr(shared), n, int(page_size), int(n_pages), at_table, width,
+                                             positions.data_ptr(), item_of_token.data_ptr(), tokens, row_start.data_ptr(),
+                                             slots.data_ptr(), taken.data_ptr(), status.data_ptr(), _stream()), "step_tables")
 
 
 class SharedPrefixPlan(NamedTuple):
@@ -1697,37 +1707,38 @@ def paged_attention_shared(q, k_cache, v_cache, positions, item_of_token, table,
     sink_values (float32 [nh]): one more term exp(value) in each head's denominator.
     plan: shared_prefix_plan() for these rows; part_acc and part_ml: the caller's scratch of plan.acc_floats and plan.ml_floats float32
     entries, not to be shared by calls that may run at the same time."""
-    _need(q.is_cuda and q.dim() == 2 and (q.shape[1] == 1 or q.stride(1) == 1), "paged_attention_shared: q [rows, heads * head size], a row's values side by side")
-    tensors = (k_cache, v_cache, positions, item_of_token, table, group_start, shared_len, out, part_acc, part_ml, status, sink_values)
-    _cuda(*tensors)
-    _here("paged_attention_shared", q, *tensors)
-    T = q.shape[0]
+    if not q.is_cuda or q.dim() != 2 or q.stride(1) != 1:
+        raise KernelError("paged_attention_shared: q [rows, heads * head size] on a CUDA device, a row's values side by side")
+    _placed("paged_attention_shared", k_cache, v_cache, positions, item_of_token, table, group_start, shared_len, out, part_acc, part_ml,
+            status, sink_values)
+    T, width = q.shape
+    code = _code(q)
+    kind = q.dtype
+    groups, splits = shared_len.numel(), plan.n_shared + plan.n_own
     _need(nkv >= 1 and nh % nkv == 0 and 16 <= hd <= 256 and hd % 16 == 0, "paged_attention_shared: heads, and head sizes of 16 to 256 in steps of 16")
-    _need(q.shape == (T, nh * hd) and out.shape == (T, nh * hd) and out.dtype == q.dtype, "paged_attention_shared: q/out shapes")
-    _need(k_cache.dtype == q.dtype and v_cache.dtype == q.dtype, "cache dtype must match q")
+    _need(width == nh * hd and out.numel() == T * width and out.dtype == kind and q.get_device() == out.get_device(),
+          "paged_attention_shared: q/out shapes, types and devices")
+    _need(k_cache.dtype == kind and v_cache.dtype == kind, "cache dtype must match q")
     _need(page_size >= 1 and n_pages >= 1 and n_pages * page_size < 1 << 31, "paged_attention_shared: pages")
     _need(min(k_cache.numel(), v_cache.numel()) >= n_pages * page_size * nkv * hd, "cache arena smaller than n_pages")
-    _need(table.dtype == torch.int32 and table.dim() == 2 and table.numel() > 0, "block table must be int32 [items, blocks]")
-    _need(positions.dtype == torch.int32 and item_of_token.dtype == torch.int32 and min(positions.numel(), item_of_token.numel()) >= T,
-          "positions / item_of_token must be int32 per row")
-    groups = shared_len.numel()
-    _need(groups >= 1 and group_start.numel() == groups + 1 and group_start.dtype == torch.int32 and shared_len.dtype == torch.int32,
-          "paged_attention_shared: group_start int32 [groups + 1], shared_len int32 [groups]")
-    _need(sink_values is None or (sink_values.dtype == torch.float32 and sink_values.numel() == nh), "sink values float32 [heads]")
+    _need(table.dim() == 2 and table.numel() > 0 and group_start.numel() == groups + 1 and groups >= 1,
+          "paged_attention_shared: table [items, blocks], group_start [groups + 1], shared_len [groups]")
+    _typed("paged_attention_shared", torch.int32, (table, 1, "table"), (positions, T, "positions"), (item_of_token, T, "item_of_token"),
+           (group_start, 2, "group_start"), (shared_len, 1, "shared_len"), (status, 4, "status"))
+    _need(plan.n_shared >= 1 and plan.n_own >= 1 and splits <= MAX_SPLITS, "paged_attention_shared: too few or too many stretches of keys")
+    _typed("paged_attention_shared", torch.float32, (part_acc, T * nh * splits * hd, "part_acc (plan.acc_floats)"),
+           (part_ml, T * nh * splits * 2, "part_ml (plan.ml_floats)"), (sink_values, nh, "sink_values"))
     _need(window is None or window >= 0, "paged_attention_shared: the window's size")
-    _need(plan.n_shared >= 1 and plan.n_own >= 1 and plan.n_shared + plan.n_own <= MAX_SPLITS, f"paged_attention_shared: 2 to {MAX_SPLITS} stretches of keys")
-    parts = T * nh * (plan.n_shared + plan.n_own)
-    _need(part_acc.dtype == torch.float32 and part_acc.numel() >= parts * hd and part_ml.dtype == torch.float32
-          and part_ml.numel() >= parts * 2, "paged_attention_shared: scratch too small for these rows and this plan")
     _need(T <= 65535 and groups <= 65535, "paged_attention_shared: at most 65535 rows and groups per launch")
     if T == 0:
         return
-    code = _code(q)
+    items, blocks = table.shape
     _check(_lib.kernels().imparo_attention_shared(
-        _ptr(q), q.stride(0) if T > 1 else nh * hd, _ptr(k_cache), _ptr(v_cache), code, _ptr(positions), _ptr(item_of_token), _ptr(table),
-        table.shape[0], table.shape[1], int(page_size), int(n_pages), _ptr(group_start), _ptr(shared_len), groups, int(window or 0),
-        float(scale), _ptr(sink_values), _ptr(out), _ptr(part_acc), _ptr(part_ml), T, nh, nkv, hd, plan.chunk_shared, plan.n_shared,
-        plan.chunk_own, plan.n_own, _ptr(status), _stream()), "paged_attention_shared")
+        q.data_ptr(), q.stride(0) if T > 1 else width, k_cache.data_ptr(), v_cache.data_ptr(), code, positions.data_ptr(),
+        item_of_token.data_ptr(), table.data_ptr(), items, blocks, int(page_size), int(n_pages), group_start.data_ptr(),
+        shared_len.data_ptr(), groups, int(window or 0), float(scale), _ptr(sink_values), out.data_ptr(), part_acc.data_ptr(),
+        part_ml.data_ptr(), T, nh, nkv, hd, plan.chunk_shared, plan.n_shared, plan.chunk_own, plan.n_own, status.data_ptr(), _stream()),
+           "paged_attention_shared")
     COUNTS["own"] += 1          # (the stretches, and what joins them)
 
 
