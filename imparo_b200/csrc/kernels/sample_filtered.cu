@@ -29,6 +29,8 @@ constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int BINS = 1024;                     // two per thread
 constexpr int LIST = 1024;                     // entries of a bin that are sorted at once
 constexpr int STAGED_MOST = 40960;             // entries of a stretch kept in shared memory (160 KB)
+constexpr int MOST_RANKS = 8;                  // CTAs of a cluster
+constexpr int FEW = 256;                       // listed entries that are compared each with each
 constexpr float BIN_RANGE = 24.0f;             // (m - v) / T covered by the bins; the last one takes all beyond
 static_assert(BINS == 2 * THREADS && LIST == 2 * THREADS, "two bins and two list entries per thread");
 
@@ -78,9 +80,7 @@ struct Weights {
     // split into a whole number n and a rest of at most 1/2; 2^(n / 64) from the table and the exponent, the rest by the first six
     // terms of the series, |r| <= ln 2 / 128: what is left out is below 2^-54.
     __device__ __forceinline__ u64 operator()(float v) const {
-        if (v == topf) return 1ull << shift;
-        const double t = ((double)v - top) * rate;
-        if (!(t > -64.0 * 64.0)) return 0;                         // below 2^-64 (and any number below an infinite one)
+        const double t = fmax(((double)v - top) * rate, -64.0 * 64.0);          // (2^-64 and less, and minus infinity: 0)
         const double whole = 6755399441055744.0;                   // 1.5 2^52: adding it rounds to a whole number
         const double tn = t + whole;
         const int n = __double2loint(tn);
@@ -88,7 +88,8 @@ struct Weights {
         const double p = fma(r, fma(r, fma(r, fma(r, fma(r, 1.0 / 120.0, 1.0 / 24.0), 1.0 / 6.0), 0.5), 1.0), 1.0);
         // times 2^(n >> 6) and 2^shift, by the exponent (at least 2^-64 2^44: a normal number)
         const double scaled = table[n & 63] * p * __hiloint2double((1023 + (n >> 6) + shift) << 20, 0);
-        return __double_as_longlong(scaled + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;        // + 2^52: rounded to a whole number
+        const u64 w = __double_as_longlong(scaled + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;       // + 2^52: rounded to a whole number
+        return v == topf ? 1ull << shift : w;                      // (the largest may be infinite)
     }
 };
 
@@ -126,6 +127,12 @@ __device__ __forceinline__ V warp_total(V v) {
     return v;
 }
 
+__device__ __forceinline__ u64 warp_largest(u64 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
 // What comes before a thread's (n, w) in thread order.  All threads call it.
 __device__ __forceinline__ void block_before(Shared& s, uint32_t n, u64 w, uint32_t& before_n, u64& before_w) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -145,24 +152,45 @@ __device__ __forceinline__ void block_before(Shared& s, uint32_t n, u64 w, uint3
     for (int i = 0; i < warp; ++i) { before_n += s.warp_n[i]; before_w += s.warp_w[i]; }
 }
 
-// Sorts list[0 .. size) falling, size a power of two up to LIST.
+// Sorts list[0 .. size) falling, size a power of two of 64 to LIST.  A bitonic network with two neighbouring entries per thread: the
+// strides within a thread or a warp are exchanged by registers, only those of 64 and more go through shared memory and a barrier.
 __device__ __forceinline__ void sort_list(u64* list, int size) {
+    const int i0 = 2 * threadIdx.x;
+    const bool active = i0 < size;                                 // (whole warps)
+    __syncthreads();
+    u64 x0 = active ? list[i0] : 0, x1 = active ? list[i0 + 1] : 0;
     for (int k = 2; k <= size; k <<= 1) {
-        for (int j = k >> 1; j > 0; j >>= 1) {
+        const bool falling = (i0 & k) == 0;
+        for (int j = k >> 1; j >= 64; j >>= 1) {
             __syncthreads();
-            const int i = threadIdx.x;
-            if (i < size / 2) {
-                const int a = 2 * j * (i / j) + i % j, b = a + j;
-                const u64 x = list[a], y = list[b];
-                if ((x < y) == ((a & k) == 0)) { list[a] = y; list[b] = x; }
+            if (active) { list[i0] = x0; list[i0 + 1] = x1; }
+            __syncthreads();
+            if (active) {
+                const u64 y0 = list[i0 ^ j], y1 = list[(i0 ^ j) + 1];
+                const bool larger = ((i0 & j) == 0) == falling;
+                x0 = larger ? max(x0, y0) : min(x0, y0);
+                x1 = larger ? max(x1, y1) : min(x1, y1);
             }
         }
+        if (active) {
+            for (int j = min(k >> 1, 32); j > 1; j >>= 1) {
+                const u64 y0 = __shfl_xor_sync(0xffffffffu, x0, j >> 1), y1 = __shfl_xor_sync(0xffffffffu, x1, j >> 1);
+                const bool larger = ((i0 & j) == 0) == falling;
+                x0 = larger ? max(x0, y0) : min(x0, y0);
+                x1 = larger ? max(x1, y1) : min(x1, y1);
+            }
+            const u64 hi = max(x0, x1), lo = min(x0, x1);
+            x0 = falling ? hi : lo;
+            x1 = falling ? lo : hi;
+        }
     }
+    __syncthreads();
+    if (active) { list[i0] = x0; list[i0 + 1] = x1; }
     __syncthreads();
 }
 
 template <typename T, bool STAGED>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 2)
 sample_filtered_kernel(const Args a) {
     extern __shared__ __align__(16) uint8_t sf_smem[];
     Shared& s = *reinterpret_cast<Shared*>(sf_smem);
@@ -207,17 +235,15 @@ sample_filtered_kernel(const Args a) {
             if (v > -INFINITY) top = max(top, entry(v, lo + i));
         }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = warp_largest(top);
     if (lane == 0) s.warp_w[warp] = top;
     __syncthreads();
-    if (tid == 0) {
-        for (int i = 1; i < WARPS; ++i) top = max(top, s.warp_w[i]);
-        s.part_top = top;
+    if (warp == 0) {
+        top = warp_largest(lane < WARPS ? s.warp_w[lane] : 0);
+        if (lane == 0) s.part_top = top;
     }
     cluster.sync();
-    top = 0;
-    for (int i = 0; i < ranks; ++i) top = max(top, *cluster.map_shared_rank(&s.part_top, i));
+    top = warp_largest(lane < ranks ? *cluster.map_shared_rank(&s.part_top, lane) : 0);           // (a lane a CTA)
 
     const float temp = a.temperature[r];
     if (top == 0 || !(temp > 0.f)) {                               // nothing to pick from, or greedy
@@ -243,33 +269,92 @@ sample_filtered_kernel(const Args a) {
         first_histogram = false;
         for (int i = tid; i < BINS; i += THREADS) { s.n[i] = 0; s.lo[i] = 0; s.hi[i] = 0; }
         __syncthreads();
-        for (int i = tid; i < count; i += THREADS) {
-            const float v = value(i);
-            const int b = take(v, lo + i);
-            if (b >= 0) {
-                atomicAdd(&s.n[b], 1u);
-                if (weights) {
-                    const u64 x = weight(v);
-                    const uint32_t low = (uint32_t)x, old = atomicAdd(&s.lo[b], low);
-                    const uint32_t high = (uint32_t)(x >> 32) + (old + low < old ? 1u : 0u);
-                    if (high) atomicAdd(&s.hi[b], high);
+        auto add_weight = [&](int b, u64 x) {
+            const uint32_t low = (uint32_t)x, old = atomicAdd(&s.lo[b], low);
+            const uint32_t high = (uint32_t)(x >> 32) + (old + low < old ? 1u : 0u);
+            if (high) atomicAdd(&s.hi[b], high);
+        };
+        // (the last bin, where the many unlikely entries fall, is counted apart: atomics on one place go one after the other)
+        uint32_t last_n = 0;
+        u64 last_w = 0;
+        for (int base = tid; base < count; base += 4 * THREADS) {  // (four at a time: a weight is a long chain of 64-bit operations)
+            int b[4];
+            u64 x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = base + j * THREADS;
+                const float v = i < count ? value(i) : -INFINITY;
+                b[j] = take(v, lo + i);
+                x[j] = weights ? weight(v) : 0;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (b[j] == BINS - 1) {
+                    ++last_n;
+                    last_w += x[j];
+                } else if (b[j] >= 0) {
+                    atomicAdd(&s.n[b[j]], 1u);
+                    if (weights) add_weight(b[j], x[j]);
                 }
             }
+        }
+        last_n = warp_total(last_n);
+        if (weights) last_w = warp_total(last_w);
+        if (lane == 0 && last_n) {
+            atomicAdd(&s.n[BINS - 1], last_n);
+            if (weights) add_weight(BINS - 1, last_w);
         }
         cluster.sync();
         n[0] = n[1] = 0;
         w[0] = w[1] = 0;
-        for (int k = 0; k < ranks; ++k) {
-            const Shared* other = cluster.map_shared_rank(&s, k);
-            const uint2 x = *reinterpret_cast<const uint2*>(&other->n[2 * tid]);
-            n[0] += x.x;
-            n[1] += x.y;
-            if (weights) {
-                const uint2 low = *reinterpret_cast<const uint2*>(&other->lo[2 * tid]), high = *reinterpret_cast<const uint2*>(&other->hi[2 * tid]);
-                w[0] += ((u64)high.x << 32) + low.x;
-                w[1] += ((u64)high.y << 32) + low.y;
+        uint2 x[MOST_RANKS];                                       // all on their way at once
+#pragma unroll
+        for (int k = 0; k < MOST_RANKS; ++k)
+            x[k] = k < ranks ? *reinterpret_cast<const uint2*>(&cluster.map_shared_rank(&s, k)->n[2 * tid]) : make_uint2(0u, 0u);
+#pragma unroll
+        for (int k = 0; k < MOST_RANKS; ++k) { n[0] += x[k].x; n[1] += x[k].y; }
+        if (weights) {
+#pragma unroll
+            for (int k = 0; k < MOST_RANKS; ++k)
+                x[k] = k < ranks ? *reinterpret_cast<const uint2*>(&cluster.map_shared_rank(&s, k)->lo[2 * tid]) : make_uint2(0u, 0u);
+#pragma unroll
+            for (int k = 0; k < MOST_RANKS; ++k) { w[0] += x[k].x; w[1] += x[k].y; }
+#pragma unroll
+            for (int k = 0; k < MOST_RANKS; ++k)
+                x[k] = k < ranks ? *reinterpret_cast<const uint2*>(&cluster.map_shared_rank(&s, k)->hi[2 * tid]) : make_uint2(0u, 0u);
+#pragma unroll
+            for (int k = 0; k < MOST_RANKS; ++k) { w[0] += (u64)x[k].x << 32; w[1] += (u64)x[k].y << 32; }
+        }
+    };
+    // The entries that `in` takes, LIST at most, into the first CTA's list, in any order.
+    auto gather = [&](auto in) {
+        Shared* first = cluster.map_shared_rank(&s, 0);
+        for (int base = tid; base - tid < count; base += 32 * THREADS) {
+            uint32_t hits = 0;
+            const int turns = min(32, (count - (base - tid) + THREADS - 1) / THREADS);
+#pragma unroll 4
+            for (int j = 0; j < turns; ++j) {
+                const int i = base + j * THREADS;
+                if (i < count && in(value(i), lo + i)) hits |= 1u << j;
+            }
+            const uint32_t mine = __popc(hits);
+            uint32_t upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += up;
+            }
+            const uint32_t all = __shfl_sync(0xffffffffu, upto, 31);
+            if (all == 0) continue;
+            uint32_t place = 0;
+            if (lane == 0) place = atomicAdd(&first->gathered, all);
+            place = __shfl_sync(0xffffffffu, place, 0) + upto - mine;
+            for (; hits; hits &= hits - 1, ++place) {
+                const int i = base + (__ffs(hits) - 1) * THREADS;
+                first->list[place] = entry(value(i), lo + i);
             }
         }
+        cluster.sync();
     };
     auto kept_bound = [&]() -> u64 {                               // min_p as a bound on the logit: w >= min_p
         if (!a.min_p || !(a.min_p[r] > 0.f)) return 1;             // (1: every number above minus infinity)
@@ -285,6 +370,52 @@ sample_filtered_kernel(const Args a) {
     // sorts it, cuts it, and picks from what stays in the order of the vocabulary.  need: the weight before which entries stay, 0:
     // top_p of the first top_k's weight, which the list holds.
     auto finish = [&](int size, u64 need) {
+        if (size <= FEW) {
+            // each entry with each: what comes before it in the order, then in the vocabulary (a sort of so few waits at its barriers
+            // for longer)
+            u64* ws = reinterpret_cast<u64*>(s.n);                 // (the histograms have been read)
+            const u64 e = tid < size ? s.list[tid] : 0;
+            const u64 x = e ? weight(unordered((uint32_t)(e >> 32))) : 0;
+            if (tid < FEW) ws[tid] = x;
+            __syncthreads();
+            uint32_t ahead = 0;
+            u64 ahead_w = 0;
+            if (warp * 32 < size) {
+#pragma unroll 4
+                for (int j = 0; j < size; ++j)
+                    if (s.list[j] > e) { ++ahead; ahead_w += ws[j]; }
+            }
+            const bool among = e != 0 && (top_k == 0 || ahead < (uint32_t)top_k);
+            uint32_t bn;
+            u64 bw;
+            if (need == 0) {
+                if (top_p < 1.f) {
+                    block_before(s, 0, among ? x : 0, bn, bw);
+                    if (tid == THREADS - 1) s.total_w = bw + (among ? x : 0);
+                    __syncthreads();
+                    need = max(part_of(top_p, s.total_w, true), 1ull);
+                } else need = ~0ull;
+            }
+            const bool stays = among && (ahead == 0 || (ahead_w < need && e >= kept_bound()));
+            __syncthreads();
+            if (tid < FEW) ws[tid] = stays ? x : 0;
+            const int stay = __syncthreads_count(stays);
+            if (stays) {
+                u64 before = 0, whole = 0;
+#pragma unroll 4
+                for (int j = 0; j < size; ++j) {
+                    const u64 y = ws[j];
+                    whole += y;
+                    if ((uint32_t)s.list[j] > (uint32_t)e) before += y;                    // (the larger is the smaller index)
+                }
+                const u64 target = target_of(a.uniform[r], whole);
+                if (before <= target && target < before + x) {
+                    a.out[r] = (int)~(uint32_t)e;
+                    if (a.kept) a.kept[r] = stay;
+                }
+            }
+            return;
+        }
         int pow2 = 64;
         while (pow2 < size) pow2 <<= 1;
         for (int i = size + tid; i < pow2; i += THREADS) s.list[i] = 0;
@@ -307,8 +438,8 @@ sample_filtered_kernel(const Args a) {
         __syncthreads();
         const int stay = max(1, (int)s.found);                     // (the first entry always stays)
         // by index: the larger key is the smaller index, with the logit behind it
-        for (int i = 0; i < 2; ++i) s.list[i0 + i] = i0 + i < stay ? (e[i] << 32) | (e[i] >> 32) : 0;
-        pow2 = 2;
+        for (int i = 0; i < 2; ++i) s.list[i0 + i] = i0 + i < stay ? (e[i] << 32) | (e[i] >> 32) : 0;        // (zeros behind them: LIST of them)
+        pow2 = 64;
         while (pow2 < stay) pow2 <<= 1;
         sort_list(s.list, pow2);
 #pragma unroll
@@ -373,19 +504,7 @@ sample_filtered_kernel(const Args a) {
             const int bin = (int)s.bin;
             const uint32_t found = s.found;
             if (level == 0 && before_n + found <= LIST) {
-                Shared* first = cluster.map_shared_rank(&s, 0);
-                for (int i = tid; i - lane < count; i += THREADS) {
-                    const float v = i < count ? value(i) : -INFINITY;
-                    const bool in = v > -INFINITY && bin_of(v) <= bin && entry(v, lo + i) >= least;
-                    const unsigned mask = __ballot_sync(0xffffffffu, in);
-                    if (mask) {
-                        uint32_t place = 0;
-                        if (lane == __ffs(mask) - 1) place = atomicAdd(&first->gathered, (uint32_t)__popc(mask));
-                        place = __shfl_sync(0xffffffffu, place, __ffs(mask) - 1) + __popc(mask & ((1u << lane) - 1u));
-                        if (in) first->list[place] = entry(v, lo + i);
-                    }
-                }
-                cluster.sync();
+                gather([&](float v, int index) { return v > -INFINITY && bin_of(v) <= bin && entry(v, index) >= least; });
                 if (rank == 0) finish((int)(before_n + found), by_rank ? 0 : need);
                 return 0;
             }
@@ -403,7 +522,7 @@ sample_filtered_kernel(const Args a) {
                 uint32_t mine = s.n[bin], first = 0;
                 for (int k = 0; k < rank; ++k) first += cluster.map_shared_rank(&s, k)->n[bin];
                 if (tid == 0) s.list_n = first;
-                int size = 32;
+                int size = 64;
                 while (size < (int)found) size <<= 1;
                 for (int i = (int)found + tid; i < size; i += THREADS) s.list[i] = 0;
                 __syncthreads();
@@ -482,11 +601,16 @@ sample_filtered_kernel(const Args a) {
     const int s0 = min(count, warp * seg), s1 = min(count, s0 + seg);
     u64 w = 0;
     uint32_t n = 0;
-    for (int i = s0 + lane; i < s1; i += 32) {
-        const float v = value(i);
-        if (v > -INFINITY && entry(v, lo + i) >= cut) {
-            w += weight(v);
-            ++n;
+    for (int base = s0 + lane; base < s1; base += 128) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = base + 32 * j;
+            const float v = i < s1 ? value(i) : -INFINITY;
+            const bool stays = v > -INFINITY && entry(v, lo + i) >= cut;
+            if (__any_sync(__activemask(), stays)) {
+                const u64 x = weight(v);
+                if (stays) { w += x; ++n; }
+            }
         }
     }
     w = warp_total(w);
@@ -494,23 +618,17 @@ sample_filtered_kernel(const Args a) {
     __syncthreads();
     if (lane == 0) { s.warp_w[warp] = w; s.warp_n[warp] = n; }
     __syncthreads();
-    if (tid == 0) {
-        u64 tw = 0;
-        uint32_t tn = 0;
-        for (int i = 0; i < WARPS; ++i) { tw += s.warp_w[i]; tn += s.warp_n[i]; }
-        s.part_w = tw;
-        s.part_n = tn;
+    if (warp == 0) {
+        const u64 tw = warp_total(lane < WARPS ? s.warp_w[lane] : 0);
+        const uint32_t tn = warp_total(lane < WARPS ? s.warp_n[lane] : 0);
+        if (lane == 0) { s.part_w = tw; s.part_n = tn; }
     }
     cluster.sync();
-    u64 before = 0, whole = 0;
-    uint32_t kept = 0;
-    for (int k = 0; k < ranks; ++k) {
-        const Shared* other = cluster.map_shared_rank(&s, k);
-        if (k < rank) before += other->part_w;
-        whole += other->part_w;
-        kept += other->part_n;
-    }
-    for (int i = 0; i < warp; ++i) before += s.warp_w[i];
+    const u64 his_w = lane < ranks ? cluster.map_shared_rank(&s, lane)->part_w : 0;
+    const uint32_t his_n = lane < ranks ? cluster.map_shared_rank(&s, lane)->part_n : 0;
+    const u64 whole = warp_total(his_w), before_cta = warp_total(lane < rank ? his_w : 0);
+    const uint32_t kept = warp_total(his_n);
+    u64 before = before_cta + warp_total(lane < warp ? s.warp_w[lane] : 0);
     const u64 target = target_of(a.uniform[r], whole);
     if (before <= target && target < before + w) {                 // (warp-uniform) this warp holds the pick
         for (int i = s0 + lane; i - lane < s1; i += 32) {
