@@ -12,12 +12,14 @@
 // one that 64-bit arithmetic gives except where a border lies within some 2^-40 of the drawn number.  In 32-bit sums, neighbours
 // with weights of 1e-5 of the total each were told apart wrongly once in some hundred rows.
 //
-// A cluster of CTAs owns a row, each CTA a contiguous stretch of it, which it keeps in shared memory: the row is read once.  The
-// cut is found by histograms over that copy (the cluster's CTAs exchange them through distributed shared memory): 1,024 bins of
-// equal width in (m - v) / T, the entries of the bin that holds the border sorted in shared memory; a bin with more entries than
-// the list holds is cut further by ten bits of the ordered logit at a time.
+// A cluster of CTAs owns a row, each CTA a contiguous stretch of it, which it keeps in shared memory where it fits; with many rows a
+// row has one CTA, which reads a long row several times, from the L2 but for the first.  The cut is found by histograms (the cluster's
+// CTAs exchange them through distributed shared memory): 1,024 bins of equal width in (m - v) / T.  Where the order up to the cut's
+// bin fits a list of 1,024 entries, the first CTA does the rest with that list alone; otherwise the entries of the cut's bin are
+// sorted, and a bin with more entries than the list holds is cut further by ten bits of the ordered logit at a time.
 #include "common.cuh"
 #include <cooperative_groups.h>
+#include <type_traits>
 
 namespace imparo {
 namespace sf {
@@ -28,9 +30,10 @@ typedef unsigned long long u64;
 constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int BINS = 1024;                     // two per thread
 constexpr int LIST = 1024;                     // entries of a bin that are sorted at once
-constexpr int STAGED_MOST = 40960;             // entries of a stretch kept in shared memory (160 KB)
+constexpr int STAGED_MOST = 16384;             // entries of a stretch kept in shared memory (64 KB: two CTAs per SM)
 constexpr int MOST_RANKS = 8;                  // CTAs of a cluster
 constexpr int FEW = 256;                       // listed entries that are compared each with each
+constexpr int LOG_STEPS = 10, STEPS = 1 << LOG_STEPS;           // of the exponential's table to a factor of two
 constexpr float BIN_RANGE = 24.0f;             // (m - v) / T covered by the bins; the last one takes all beyond
 static_assert(BINS == 2 * THREADS && LIST == 2 * THREADS, "two bins and two list entries per thread");
 
@@ -49,12 +52,14 @@ struct Args {
 
 struct Shared {
     uint32_t n[BINS], lo[BINS], hi[BINS];                          // this CTA's histogram: counts, weights in two halves
+    uint32_t all_n[BINS];                                          // the cluster's, written share by share by its CTAs
+    u64 all_w[BINS];
     u64 list[LIST];                                                // entries that are sorted
-    double table[64];                                              // 2^(i / 64)
+    double table[STEPS];                                           // 2^(i / STEPS)
     u64 warp_w[WARPS + 1];
     uint32_t warp_n[WARPS + 1];
-    u64 part_top, part_w;                                          // read by the other CTAs
-    uint32_t part_n, list_n, gathered;
+    u64 part_w;                                                    // read by the other CTAs
+    uint32_t part_n, list_n, gathered[2];      // (the first: the same in every CTA)
     u64 before_w, found_cut, total_w;
     uint32_t before_n, bin, found, total_n;
 };
@@ -68,28 +73,32 @@ __device__ __forceinline__ float unordered(uint32_t k) { return __uint_as_float(
 // an entry's place in the order as one number: the larger comes first
 __device__ __forceinline__ u64 entry(float v, int index) { return ((u64)ordered(v) << 32) | (uint32_t)~index; }
 
+// the place in the order at or above which every number above minus infinity lies
+constexpr u64 ALL = (u64)0x00800000u << 32;
+
 // NaN is no number: it is taken for minus infinity, which no filter keeps
 __device__ __forceinline__ float clean(float v) { return v == v ? v + 0.0f : -INFINITY; }
 
 struct Weights {
-    double top, rate;          // the row's largest logit; 64 log2(e) / T
-    const double* table;
-    float topf;
+    double top, rate;          // the row's largest logit; STEPS log2(e) / T
+    const double* table;       // 2^(i / STEPS)
+    float topf, least;         // below `least` a weight is 0
     int shift;
-    // exp((v - top) / T) as a multiple of 2^-shift.  Table-driven exponential (P. T. P. Tang, 1989): t = 64 log2(e) (v - top) / T is
-    // split into a whole number n and a rest of at most 1/2; 2^(n / 64) from the table and the exponent, the rest by the first six
-    // terms of the series, |r| <= ln 2 / 128: what is left out is below 2^-54.
+    // exp((v - top) / T), v above minus infinity, as a multiple of 2^-shift.  Table-driven exponential (P. T. P. Tang, 1989): t =
+    // STEPS log2(e) (v - top) / T is split into a whole number n and a rest f of at most 1/2; 2^(n / STEPS) from the table and the
+    // exponent, 2^(f / STEPS) by its series in f: with 1,024 steps the first four terms leave out less than 2^-50.
     __device__ __forceinline__ u64 operator()(float v) const {
-        const double t = fmax(((double)v - top) * rate, -64.0 * 64.0);          // (2^-64 and less, and minus infinity: 0)
+        const double t = ((double)v - top) * rate;
         const double whole = 6755399441055744.0;                   // 1.5 2^52: adding it rounds to a whole number
         const double tn = t + whole;
         const int n = __double2loint(tn);
-        const double r = (t - (tn - whole)) * (0.69314718055994530942 / 64.0);
-        const double p = fma(r, fma(r, fma(r, fma(r, fma(r, 1.0 / 120.0, 1.0 / 24.0), 1.0 / 6.0), 0.5), 1.0), 1.0);
-        // times 2^(n >> 6) and 2^shift, by the exponent (at least 2^-64 2^44: a normal number)
-        const double scaled = table[n & 63] * p * __hiloint2double((1023 + (n >> 6) + shift) << 20, 0);
-        const u64 w = __double_as_longlong(scaled + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;       // + 2^52: rounded to a whole number
-        return v == topf ? 1ull << shift : w;                      // (the largest may be infinite)
+        const double f = t - (tn - whole);
+        constexpr double c = 0.69314718055994530942 / STEPS;
+        const double p = table[n & (STEPS - 1)] * fma(f, fma(f, fma(f, c * c * c / 6.0, c * c / 2.0), c), 1.0);
+        // times 2^(n / STEPS) and 2^shift, by the exponent (from 2^-63 2^38 on: a normal number), then + 2^52: rounded to a whole one
+        const double scaled = __hiloint2double(__double2hiint(p) + (((n >> LOG_STEPS) + shift) << 20), __double2loint(p));
+        const u64 w = __double_as_longlong(scaled + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+        return v == topf ? 1ull << shift : v < least ? 0 : w;      // (the largest may be infinite)
     }
 };
 
@@ -116,6 +125,15 @@ __device__ __forceinline__ u64 part_of(float x, u64 num, bool up) {
 
 // The weight that the running sum has to pass for the pick.  (The largest entry always stays: total >= 1.)
 __device__ __forceinline__ u64 target_of(float u, u64 total) { return u < 1.f ? (u > 0.f ? part_of(u, total, false) : 0) : total - 1; }
+
+// where four logits lie
+struct Places {
+    int first, step;
+    __device__ __forceinline__ int operator()(int e) const { return first + e * step; }
+};
+template <typename T> struct Four;
+template <> struct Four<float> { using type = uint4; };
+template <> struct Four<__nv_bfloat16> { using type = uint2; };
 
 template <typename T>
 __device__ __forceinline__ float load1(const T* p) { return clean(to_f32(*p)); }
@@ -203,68 +221,186 @@ sample_filtered_kernel(const Args a) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int lo = min(a.vocab, rank * a.per), count = min(a.vocab, lo + a.per) - lo;
     const T* row = reinterpret_cast<const T*>(a.logits) + (size_t)r * a.ld + lo;
+    // A warp owns a contiguous part of the stretch, so the warps' sums are in the order of the vocabulary.
+    constexpr int VEC = 16 / sizeof(T);
+    const int seg = ((count + WARPS - 1) / WARPS + 7) / 8 * 8, s0 = min(count, warp * seg), s1 = min(count, s0 + seg);
+    const bool aligned = ((uintptr_t)row & 15) == 0;
     auto value = [&](int i) -> float { return STAGED ? staged[i] : load1(row + i); };
+    // f(four logits, their places in the stretch) over a part of it by one warp, the next four on their way meanwhile; places at or
+    // beyond `to` come as minus infinity.
+    auto visit = [&](int from, int to, auto f) __attribute__((always_inline)) {
+        if (STAGED) {
+            for (int i = from + 4 * lane; i < to; i += 128) {      // (from is a multiple of 8; behind the stretch lie minus infinities)
+                const float4 x = *reinterpret_cast<const float4*>(staged + i);
+                const float v[4] = {x.x, i + 1 < to ? x.y : -INFINITY, i + 2 < to ? x.z : -INFINITY, i + 3 < to ? x.w : -INFINITY};
+                f(v, Places{i, 1});
+            }
+        } else if (aligned) {
+            using Raw = typename Four<T>::type;
+            const int whole = to & ~3;                             // (from is a multiple of 8)
+            int i = from + 4 * lane;
+            Raw raw{}, next{};
+            if (i < whole) raw = *reinterpret_cast<const Raw*>(row + i);
+            for (; i < whole; i += 128) {
+                if (i + 128 < whole) next = *reinterpret_cast<const Raw*>(row + i + 128);
+                const T* x = reinterpret_cast<const T*>(&raw);
+                const float v[4] = {clean(to_f32(x[0])), clean(to_f32(x[1])), clean(to_f32(x[2])), clean(to_f32(x[3]))};
+                f(v, Places{i, 1});
+                raw = next;
+            }
+            if (whole < to) {                                      // the last ones, by the first lanes
+                const float v[4] = {whole + lane < to ? load1(row + whole + lane) : -INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                f(v, Places{whole + lane, 32});
+            }
+        } else {
+            for (int i = from + lane; i < to; i += 128) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = i + 32 * e < to ? load1(row + i + 32 * e) : -INFINITY;
+                f(v, Places{i, 32});
+            }
+        }
+    };
+    // f(logit, place) for those of a part that `pick` takes: few
+    auto visit_some = [&](int from, int to, auto pick, auto f) __attribute__((always_inline)) {
+        visit(from, to, [&](const float (&v)[4], Places at) {
+            uint32_t hits = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) hits |= pick(v[e], at(e)) ? 1u << e : 0u;
+            for (; hits; hits &= hits - 1) {
+                const int i = at(__ffs(hits) - 1);
+                f(value(i), i);
+            }
+        });
+    };
 
-    if (tid < 64) s.table[tid] = exp2((double)tid / 64.0);
-    if (tid == 0) s.gathered = 0;
+    for (int i = tid; i < STEPS; i += THREADS) s.table[i] = exp2((double)i / STEPS);
+    if (tid < 2) s.gathered[tid] = 0;
 
-    // ---- the stretch into shared memory, its first largest entry ----
-    u64 top = 0;                                                   // (0: no number above minus infinity)
+    // ---- the stretch into shared memory, every thread's first largest entry ----
+    u64 mine = 0;                                                  // (0: no number above minus infinity)
     {
-        constexpr int VEC = 16 / sizeof(T);
+        float most = -INFINITY;
+        int place = 0;
+        auto look = [&](float v, int i) {
+            if (v > most) { most = v; place = i; }
+        };
         int done = 0;
-        if (STAGED && ((uintptr_t)row & 15) == 0) {
+        if (aligned) {
             const int vecs = count / VEC;
             const uint4* src = reinterpret_cast<const uint4*>(row);
-#pragma unroll 4
-            for (int i = tid; i < vecs; i += THREADS) {
-                const uint4 raw = src[i];
-                const T* x = reinterpret_cast<const T*>(&raw);
+            for (int i = tid; i < vecs; i += 4 * THREADS) {
+                uint4 raw[4];                                      // 64 bytes a thread on their way at once
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float v = clean(to_f32(x[e]));
-                    staged[i * VEC + e] = v;
-                    if (v > -INFINITY) top = max(top, entry(v, lo + i * VEC + e));
+                for (int u = 0; u < 4; ++u) raw[u] = i + u * THREADS < vecs ? src[i + u * THREADS] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (i + u * THREADS >= vecs) break;
+                    const T* x = reinterpret_cast<const T*>(&raw[u]);
+                    const int at = (i + u * THREADS) * VEC;
+#pragma unroll
+                    for (int e = 0; e < VEC; e += 4) {
+                        float4 v;
+                        v.x = clean(to_f32(x[e])); v.y = clean(to_f32(x[e + 1])); v.z = clean(to_f32(x[e + 2])); v.w = clean(to_f32(x[e + 3]));
+                        look(v.x, at + e); look(v.y, at + e + 1); look(v.z, at + e + 2); look(v.w, at + e + 3);
+                        if (STAGED) *reinterpret_cast<float4*>(staged + at + e) = v;
+                    }
                 }
             }
             done = vecs * VEC;
         }
-        for (int i = done + tid; i < count; i += THREADS) {
-            const float v = load1(row + i);
+        for (int i = done + tid; i < (STAGED ? a.per : count); i += THREADS) {
+            const float v = i < count ? load1(row + i) : -INFINITY;
             if (STAGED) staged[i] = v;
-            if (v > -INFINITY) top = max(top, entry(v, lo + i));
+            look(v, i);
         }
+        if (most > -INFINITY) mine = entry(most, lo + place);
     }
+    // The largest entries of 512 to 1,024 groups that share no entry, in every CTA: the k-th largest of them is a place at or above
+    // which at least k entries of the row lie, and not many more while k is well below the number of groups.
+    u64* largest = reinterpret_cast<u64*>(s.n);                    // (before the first histogram)
+    const int groups = ranks == 1 ? THREADS : 2 * THREADS;
+    {
+        const int group = ranks > 2 ? ranks / 2 : 1;               // threads that share one
+        for (int o = 1; o < group; o <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+        if (tid % group == 0)
+            for (int k = 0; k < ranks; ++k) *cluster.map_shared_rank(&largest[rank * (groups / ranks) + tid / group], k) = mine;
+    }
+    cluster.sync();
+    const float temp = a.temperature[r];
+    const int top_k = a.top_k && a.top_k[r] > 0 && a.top_k[r] < a.vocab ? a.top_k[r] : 0;          // 0: all
+    const float top_p = a.top_p && a.top_p[r] < 1.f ? fmaxf(a.top_p[r], 0.f) : 1.f;                // 1: all
+    u64 top = 0, from = 0;                                         // the row's first largest entry; where a list of candidates begins
+    for (int i = tid; i < groups; i += THREADS) top = max(top, largest[i]);
     top = warp_largest(top);
     if (lane == 0) s.warp_w[warp] = top;
     __syncthreads();
-    if (warp == 0) {
-        top = warp_largest(lane < WARPS ? s.warp_w[lane] : 0);
-        if (lane == 0) s.part_top = top;
+    top = warp_largest(lane < WARPS ? s.warp_w[lane] : 0);
+    // About -groups log(1 - k / groups) entries of rows without order lie at or above the k-th of the groups' largest: 720 at 386 of
+    // 512 and 516 of 1,024, which the list takes with room to spare.
+    const int likely = ranks == 1 ? 386 : 516;
+    if (temp > 0.f && top_k > 0 && top_k <= groups) {
+        // the upper 22 bits of its logit are enough, the lowest logit of those bits is below it by less than 2^-13 of itself
+        const uint32_t x0 = (uint32_t)(largest[tid] >> 32), x1 = ranks == 1 ? 0 : (uint32_t)(largest[tid + THREADS] >> 32);
+        uint32_t key = 0;
+        for (uint32_t bit = 1u << 31; bit >= 1u << 10; bit >>= 1) {
+            const uint32_t trial = key | bit;
+            const int n = __syncthreads_count(x0 >= trial) + (ranks == 1 ? 0 : __syncthreads_count(x1 >= trial));
+            if (n >= top_k) key = trial;
+        }
+        from = (u64)key << 32;                                     // (0: fewer groups than top_k have an entry)
     }
-    cluster.sync();
-    top = warp_largest(lane < ranks ? *cluster.map_shared_rank(&s.part_top, lane) : 0);           // (a lane a CTA)
+    if (temp > 0.f && top_p >= 1.f && top_k == 0 && a.min_p && a.min_p[r] > 0.f) from = ALL;       // (min_p alone)
+    if (a.vocab <= LIST && (top_k > 0 || top_p < 1.f)) from = max(from, ALL);
+    __syncthreads();                                               // (the histograms take the groups' place)
 
-    const float temp = a.temperature[r];
     if (top == 0 || !(temp > 0.f)) {                               // nothing to pick from, or greedy
         if (rank == 0 && tid == 0) {
             a.out[r] = top == 0 ? 0 : (int)~(uint32_t)top;
             if (a.kept) a.kept[r] = top == 0 ? 0 : 1;
         }
-        cluster.sync();                                            // no CTA ends while another reads its shared memory
-        return;
+        return;                                                    // (no CTA looks into another from here on)
     }
     const float topf = unordered((uint32_t)(top >> 32));
     Weights weight;
-    weight.top = topf; weight.topf = topf; weight.rate = 64.0 * 1.4426950408889634074 / (double)temp; weight.table = s.table;
+    weight.top = topf; weight.topf = topf; weight.rate = STEPS * 1.4426950408889634074 / (double)temp; weight.least = topf - 43.5f * temp; weight.table = s.table;
     weight.shift = a.shift;
-    const float per_bin = (float)BINS / (BIN_RANGE * temp);
+    // Entries below floor_v lie beyond every cut: the last bin is theirs.
+    float floor_v = from > ALL ? unordered((uint32_t)(from >> 32)) : -INFINITY;
+    if (top_k == 0 && top_p < 1.f) {
+        // all weigh at least what the groups' largest weigh, M; entries of at most (1 - top_p) M / vocab weigh at most (1 - top_p) of
+        // all together, so top_p is reached before them
+        u64 w = 0;
+        for (int i = tid; i < groups; i += THREADS) w += largest[i] ? weight(unordered((uint32_t)(largest[i] >> 32))) : 0;
+        w = warp_total(w);
+        __syncthreads();
+        if (lane == 0) s.warp_w[warp] = w;
+        __syncthreads();
+        w = warp_total(lane < WARPS ? s.warp_w[lane] : 0);
+        const double least_w = (double)((w - part_of(top_p, w, true)) / (u64)a.vocab) * exp2(-(double)a.shift);
+        // (less by far more than the logarithm's and the product's rounding)
+        floor_v = __double2float_rd((double)topf + (double)temp * (log(least_w) - 1e-9) - 1e-9 * fabs((double)topf));
+        if (!(floor_v <= topf)) floor_v = -INFINITY;
+        __syncthreads();                                           // (the histograms take the groups' place)
+    }
+    const float per_bin = floor_v > -INFINITY && floor_v < topf && topf < INFINITY ? (float)(BINS - 1) / (topf - floor_v) : (float)BINS / (BIN_RANGE * temp);
     // the bin of a logit: never falls as the logit falls, whatever the rounding
-    auto bin_of = [&](float v) -> int { return v == topf ? 0 : min(BINS - 1, (int)((topf - v) * per_bin)); };
+    auto bin_of = [&](float v) -> int {                            // (rounded down by adding 2^23)
+        const int b = __float_as_int(__fadd_rz(fminf((topf - v) * per_bin, (float)(BINS - 1)), 8388608.0f)) & (BINS - 1);
+        return v == topf ? 0 : v < floor_v ? BINS - 1 : b;
+    };
+    // whether an entry lies at or above a place in the order
+    auto at_least = [&](float v, int index, u64 place) -> bool {
+        const float pv = unordered((uint32_t)(place >> 32));
+        return v > pv || (v == pv && (uint32_t)index <= ~(uint32_t)place);
+    };
+
+    auto kept_weight = [&](float v, int i, u64 cut) -> u64 { return v > -INFINITY && at_least(v, lo + i, cut) ? weight(v) : 0; };
 
     // The cluster's histogram over the entries that `take` maps to a bin (-1: none): a thread gets its two bins' sums.
     bool first_histogram = true;
-    auto histogram = [&](bool weights, auto take, uint32_t (&n)[2], u64 (&w)[2]) {
+    auto histogram = [&](auto weighed, auto take, uint32_t (&n)[2], u64 (&w)[2]) __attribute__((always_inline)) {
+        constexpr bool weights = decltype(weighed)::value;
         if (!first_histogram) cluster.sync();                      // the others have read the one before
         first_histogram = false;
         for (int i = tid; i < BINS; i += THREADS) { s.n[i] = 0; s.lo[i] = 0; s.hi[i] = 0; }
@@ -277,27 +413,23 @@ sample_filtered_kernel(const Args a) {
         // (the last bin, where the many unlikely entries fall, is counted apart: atomics on one place go one after the other)
         uint32_t last_n = 0;
         u64 last_w = 0;
-        for (int base = tid; base < count; base += 4 * THREADS) {  // (four at a time: a weight is a long chain of 64-bit operations)
+        visit(s0, s1, [&](const float (&v)[4], Places at) {
             int b[4];
-            u64 x[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int i = base + j * THREADS;
-                const float v = i < count ? value(i) : -INFINITY;
-                b[j] = take(v, lo + i);
-                x[j] = weights ? weight(v) : 0;
+            for (int e = 0; e < 4; ++e) {
+                b[e] = take(v[e], lo + at(e));
+                if (b[e] == BINS - 1) ++last_n;
+                else if (b[e] >= 0) atomicAdd(&s.n[b[e]], 1u);
             }
+            if (weights) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (b[j] == BINS - 1) {
-                    ++last_n;
-                    last_w += x[j];
-                } else if (b[j] >= 0) {
-                    atomicAdd(&s.n[b[j]], 1u);
-                    if (weights) add_weight(b[j], x[j]);
+                for (int e = 0; e < 4; ++e) {
+                    const u64 x = weight(v[e]);
+                    if (b[e] == BINS - 1) last_w += x;
+                    else if (b[e] >= 0) add_weight(b[e], x);
                 }
             }
-        }
+        });
         last_n = warp_total(last_n);
         if (weights) last_w = warp_total(last_w);
         if (lane == 0 && last_n) {
@@ -305,66 +437,64 @@ sample_filtered_kernel(const Args a) {
             if (weights) add_weight(BINS - 1, last_w);
         }
         cluster.sync();
-        n[0] = n[1] = 0;
-        w[0] = w[1] = 0;
-        uint2 x[MOST_RANKS];                                       // all on their way at once
+        if (ranks == 1) {
 #pragma unroll
-        for (int k = 0; k < MOST_RANKS; ++k)
-            x[k] = k < ranks ? *reinterpret_cast<const uint2*>(&cluster.map_shared_rank(&s, k)->n[2 * tid]) : make_uint2(0u, 0u);
-#pragma unroll
-        for (int k = 0; k < MOST_RANKS; ++k) { n[0] += x[k].x; n[1] += x[k].y; }
-        if (weights) {
-#pragma unroll
-            for (int k = 0; k < MOST_RANKS; ++k)
-                x[k] = k < ranks ? *reinterpret_cast<const uint2*>(&cluster.map_shared_rank(&s, k)->lo[2 * tid]) : make_uint2(0u, 0u);
-#pragma unroll
-            for (int k = 0; k < MOST_RANKS; ++k) { w[0] += x[k].x; w[1] += x[k].y; }
-#pragma unroll
-            for (int k = 0; k < MOST_RANKS; ++k)
-                x[k] = k < ranks ? *reinterpret_cast<const uint2*>(&cluster.map_shared_rank(&s, k)->hi[2 * tid]) : make_uint2(0u, 0u);
-#pragma unroll
-            for (int k = 0; k < MOST_RANKS; ++k) { w[0] += (u64)x[k].x << 32; w[1] += (u64)x[k].y << 32; }
+            for (int i = 0; i < 2; ++i) {
+                n[i] = s.n[2 * tid + i];
+                w[i] = weights ? ((u64)s.hi[2 * tid + i] << 32) + s.lo[2 * tid + i] : 0;
+            }
+            return;
         }
+        // a CTA sums its share of the bins and gives the sums to all (each summing all bins reads eight times as much from the others)
+        const int share = BINS / ranks;
+        for (int i = rank * share + tid; i < (rank + 1) * share; i += THREADS) {
+            uint32_t sum_n = 0;
+            u64 sum_w = 0;
+            uint32_t x[MOST_RANKS];                                // all on their way at once
+#pragma unroll
+            for (int k = 0; k < MOST_RANKS; ++k) x[k] = k < ranks ? cluster.map_shared_rank(&s, k)->n[i] : 0;
+#pragma unroll
+            for (int k = 0; k < MOST_RANKS; ++k) sum_n += x[k];
+            if (weights) {
+                uint32_t y[MOST_RANKS];
+#pragma unroll
+                for (int k = 0; k < MOST_RANKS; ++k) {
+                    x[k] = k < ranks ? cluster.map_shared_rank(&s, k)->lo[i] : 0;
+                    y[k] = k < ranks ? cluster.map_shared_rank(&s, k)->hi[i] : 0;
+                }
+#pragma unroll
+                for (int k = 0; k < MOST_RANKS; ++k) sum_w += ((u64)y[k] << 32) + x[k];
+            }
+            for (int k = 0; k < ranks; ++k) {
+                Shared* other = cluster.map_shared_rank(&s, k);
+                other->all_n[i] = sum_n;
+                if (weights) other->all_w[i] = sum_w;
+            }
+        }
+        cluster.sync();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) { n[i] = s.all_n[2 * tid + i]; w[i] = weights ? s.all_w[2 * tid + i] : 0; }
     };
     // The entries that `in` takes, LIST at most, into the first CTA's list, in any order.
     auto gather = [&](auto in) {
         Shared* first = cluster.map_shared_rank(&s, 0);
-        for (int base = tid; base - tid < count; base += 32 * THREADS) {
-            uint32_t hits = 0;
-            const int turns = min(32, (count - (base - tid) + THREADS - 1) / THREADS);
-#pragma unroll 4
-            for (int j = 0; j < turns; ++j) {
-                const int i = base + j * THREADS;
-                if (i < count && in(value(i), lo + i)) hits |= 1u << j;
-            }
-            const uint32_t mine = __popc(hits);
-            uint32_t upto = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += up;
-            }
-            const uint32_t all = __shfl_sync(0xffffffffu, upto, 31);
-            if (all == 0) continue;
+        visit_some(s0, s1, [&](float v, int i) { return in(v, lo + i); }, [&](float v, int i) {
+            const unsigned here = __activemask();                  // (the lanes that are here together ask once)
+            const int leader = __ffs(here) - 1;
             uint32_t place = 0;
-            if (lane == 0) place = atomicAdd(&first->gathered, all);
-            place = __shfl_sync(0xffffffffu, place, 0) + upto - mine;
-            for (; hits; hits &= hits - 1, ++place) {
-                const int i = base + (__ffs(hits) - 1) * THREADS;
-                first->list[place] = entry(value(i), lo + i);
-            }
-        }
+            if (lane == leader) place = atomicAdd(&first->gathered[1], (uint32_t)__popc(here));
+            place = __shfl_sync(here, place, leader) + __popc(here & ((1u << lane) - 1u));
+            first->list[place] = entry(v, lo + i);
+        });
         cluster.sync();
     };
     auto kept_bound = [&]() -> u64 {                               // min_p as a bound on the logit: w >= min_p
-        if (!a.min_p || !(a.min_p[r] > 0.f)) return 1;             // (1: every number above minus infinity)
+        if (!a.min_p || !(a.min_p[r] > 0.f)) return ALL;
         const float p = a.min_p[r];
         if (p > 1.f) return top;                                   // only the first largest entry stays
         const float bound = __double2float_ru((double)topf + (double)temp * log((double)p));
-        return bound > -INFINITY ? (u64)ordered(bound + 0.0f) << 32 : 1;
+        return bound > -INFINITY ? (u64)ordered(bound + 0.0f) << 32 : ALL;
     };
-    const int top_k = a.top_k && a.top_k[r] > 0 && a.top_k[r] < a.vocab ? a.top_k[r] : 0;          // 0: all
-    const float top_p = a.top_p && a.top_p[r] < 1.f ? fmaxf(a.top_p[r], 0.f) : 1.f;                // 1: all
 
     // All that is left to do, by the first CTA alone, where the list holds a beginning of the order that reaches beyond every cut:
     // sorts it, cuts it, and picks from what stays in the order of the vocabulary.  need: the weight before which entries stay, 0:
@@ -437,31 +567,32 @@ sample_filtered_kernel(const Args a) {
         if (e[1] && bw + x[0] < need && e[1] >= bound) atomicMax(&s.found, (uint32_t)i0 + 2);
         __syncthreads();
         const int stay = max(1, (int)s.found);                     // (the first entry always stays)
-        // by index: the larger key is the smaller index, with the logit behind it
-        for (int i = 0; i < 2; ++i) s.list[i0 + i] = i0 + i < stay ? (e[i] << 32) | (e[i] >> 32) : 0;        // (zeros behind them: LIST of them)
-        pow2 = 64;
-        while (pow2 < stay) pow2 <<= 1;
-        sort_list(s.list, pow2);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) x[i] = i0 + i < stay ? weight(unordered((uint32_t)s.list[i0 + i])) : 0;
-        block_before(s, 0, x[0] + x[1], bn, bw);
-        if (tid == THREADS - 1) s.total_w = bw + x[0] + x[1];
-        __syncthreads();
-        const u64 target = target_of(a.uniform[r], s.total_w);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (bw <= target && target < bw + x[i]) {
-                a.out[r] = (int)~(uint32_t)(s.list[i0 + i] >> 32);
-                if (a.kept) a.kept[r] = stay;
-            }
-            bw += x[i];
+        // The pick: the smallest index up to which more than the target weighs, bit by bit of its complement (which e holds), from
+        // the top: entries whose complement is at least `trial` are those up to an index.
+        const bool in0 = i0 < stay, in1 = i0 + 1 < stay;
+        const uint32_t c0 = (uint32_t)e[0], c1 = (uint32_t)e[1];
+        auto weight_from = [&](uint32_t least) -> u64 {
+            u64 w = warp_total((in0 && c0 >= least ? x[0] : 0) + (in1 && c1 >= least ? x[1] : 0));
+            __syncthreads();
+            if (lane == 0) s.warp_w[warp] = w;
+            __syncthreads();
+            return warp_total(lane < WARPS ? s.warp_w[lane] : 0);
+        };
+        const u64 target = target_of(a.uniform[r], weight_from(0));
+        uint32_t least = 0xff000000u;                              // (indexes have 24 bits)
+        for (uint32_t bit = 1u << 23; bit != 0; bit >>= 1)
+            if (weight_from(least | bit) > target) least |= bit;   // the largest complement from which on enough weighs
+        if ((in0 && c0 == least) || (in1 && c1 == least)) {
+            a.out[r] = (int)~least;
+            if (a.kept) a.kept[r] = stay;
         }
     };
 
     // The cut behind the last entry kept: entries are counted (by_rank: the first top_k of the order stay) or weighed (those stay before
     // which less than top_p of the total weighs), over the entries at or above `least`.  Returns 0 where the first CTA has finished
     // the row: the beginning of the order up to the cut's bin fits the list.
-    auto find_cut = [&](bool by_rank, u64 least) -> u64 {
+    auto find_cut = [&](auto counted, u64 least) __attribute__((always_inline)) -> u64 {
+        constexpr bool by_rank = decltype(counted)::value;
         u64 need = by_rank ? (u64)top_k : 0;
         uint32_t before_n = 0;
         u64 before_w = 0;
@@ -472,8 +603,8 @@ sample_filtered_kernel(const Args a) {
             const int down = level == 0 ? 32 : level < 4 ? 32 - 10 * level : 0, up = level == 1 ? 0 : 42 - 10 * level;
             uint32_t hn[2];
             u64 hw[2];
-            histogram(!by_rank, [&](float v, int index) -> int {
-                if (!(v > -INFINITY) || entry(v, index) < least) return -1;
+            histogram(std::bool_constant<!by_rank>{}, [&](float v, int index) -> int {
+                if (!(v > -INFINITY) || !at_least(v, index, least)) return -1;
                 const int b = bin_of(v);
                 if (level == 0) return b;
                 const uint32_t k = ordered(v);
@@ -504,7 +635,7 @@ sample_filtered_kernel(const Args a) {
             const int bin = (int)s.bin;
             const uint32_t found = s.found;
             if (level == 0 && before_n + found <= LIST) {
-                gather([&](float v, int index) { return v > -INFINITY && bin_of(v) <= bin && entry(v, index) >= least; });
+                gather([&](float v, int index) { return v > -INFINITY && bin_of(v) <= bin && at_least(v, index, least); });
                 if (rank == 0) finish((int)(before_n + found), by_rank ? 0 : need);
                 return 0;
             }
@@ -512,7 +643,7 @@ sample_filtered_kernel(const Args a) {
             else prefix = level == 4 ? prefix : (level == 1 ? 0u : prefix << 10) | (uint32_t)(BINS - 1 - bin);
             const uint32_t last_digit = level == 4 ? (uint32_t)(BINS - 1 - bin) : 0u;
             auto in_set = [&](float v, int index) -> bool {
-                if (!(v > -INFINITY) || entry(v, index) < least || bin_of(v) != chosen_bin) return false;
+                if (!(v > -INFINITY) || !at_least(v, index, least) || bin_of(v) != chosen_bin) return false;
                 const uint32_t k = ordered(v);
                 if (level == 4) return k == ((prefix << 2) | last_digit);
                 return level == 0 || (k >> down) == prefix;
@@ -527,13 +658,10 @@ sample_filtered_kernel(const Args a) {
                 for (int i = (int)found + tid; i < size; i += THREADS) s.list[i] = 0;
                 __syncthreads();
                 if (mine) {
-                    for (int i = tid; i < count; i += THREADS) {
-                        const float v = value(i);
-                        if (in_set(v, lo + i)) {
-                            const uint32_t at_list = atomicAdd(&s.list_n, 1u);
-                            for (int k = 0; k < ranks; ++k) cluster.map_shared_rank(&s, k)->list[at_list] = entry(v, lo + i);
-                        }
-                    }
+                    visit_some(s0, s1, [&](float v, int i) { return in_set(v, lo + i); }, [&](float v, int i) {
+                        const uint32_t at_list = atomicAdd(&s.list_n, 1u);
+                        for (int k = 0; k < ranks; ++k) cluster.map_shared_rank(&s, k)->list[at_list] = entry(v, lo + i);
+                    });
                 }
                 cluster.sync();
                 sort_list(s.list, size);
@@ -558,10 +686,11 @@ sample_filtered_kernel(const Args a) {
                     const u64 w = weight(v);
                     stay = w ? min((u64)found, (need - before_w + w - 1) / w) : found;
                 }
-                const int seg = ((count + WARPS - 1) / WARPS + 31) / 32 * 32;
-                const int s0 = min(count, warp * seg), s1 = min(count, s0 + seg);
                 uint32_t n = 0;
-                for (int i = s0 + lane; i < s1; i += 32) n += in_set(value(i), lo + i) ? 1u : 0u;
+                visit(s0, s1, [&](const float (&v)[4], Places at) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) n += in_set(v[e], lo + at(e)) ? 1u : 0u;
+                });
                 n = warp_total(n);
                 __syncthreads();
                 if (lane == 0) s.warp_n[warp] = n;
@@ -591,28 +720,53 @@ sample_filtered_kernel(const Args a) {
         }
     };
 
-    u64 cut = 1;                                                   // every number above minus infinity
-    if (top_k > 0 && (cut = find_cut(true, cut)) == 0) return;
-    if (top_p < 1.f && (cut = find_cut(false, cut)) == 0) return;
-    cut = max(cut, kept_bound());
-
-    // ---- the kept weights in vocabulary order: warps own contiguous stretches, whose sums are whole numbers ----
-    const int seg = ((count + WARPS - 1) / WARPS + 31) / 32 * 32;
-    const int s0 = min(count, warp * seg), s1 = min(count, s0 + seg);
-    u64 w = 0;
-    uint32_t n = 0;
-    for (int base = s0 + lane; base < s1; base += 128) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int i = base + 32 * j;
-            const float v = i < s1 ? value(i) : -INFINITY;
-            const bool stays = v > -INFINITY && entry(v, lo + i) >= cut;
-            if (__any_sync(__activemask(), stays)) {
-                const u64 x = weight(v);
-                if (stays) { w += x; ++n; }
+    // ---- a list of candidates: a beginning of the order that reaches beyond every cut, if it is short enough ----
+    if (from != 0 && (top_k <= likely || a.vocab <= LIST)) {
+        from = max(from, top_p >= 1.f ? kept_bound() : ALL);       // (top_p is of all that top_k leaves)
+        Shared* first = cluster.map_shared_rank(&s, 0);
+        visit_some(s0, s1, [&](float v, int i) { return at_least(v, lo + i, from); }, [&](float v, int i) {
+            if (*reinterpret_cast<volatile uint32_t*>(&s.gathered[0]) > LIST) return;          // (too many: every CTA will find so)
+            const unsigned here = __activemask();                  // (the lanes that are here together ask once)
+            const int leader = __ffs(here) - 1;
+            uint32_t place = 0;
+            if (lane == leader) {
+                place = atomicAdd(&first->gathered[0], (uint32_t)__popc(here));
+                for (int k = 1; k < ranks; ++k) atomicAdd(&cluster.map_shared_rank(&s, k)->gathered[0], (uint32_t)__popc(here));
             }
+            place = __shfl_sync(here, place, leader) + __popc(here & ((1u << lane) - 1u));
+            if (place < LIST) first->list[place] = entry(v, lo + i);
+        });
+        cluster.sync();
+        if (s.gathered[0] <= LIST) {
+            if (rank == 0) finish((int)s.gathered[0], 0);
+            return;
         }
     }
+
+    // ---- cuts that lie further down: by histograms ----
+    u64 cut = ALL;
+    if (top_k > 0 && (cut = find_cut(std::true_type{}, cut)) == 0) return;
+    if (top_p < 1.f && (cut = find_cut(std::false_type{}, cut)) == 0) return;
+    cut = max(cut, kept_bound());
+
+    // ---- the kept weights in vocabulary order: warps own contiguous parts, whose sums are whole numbers ----
+    u64 w = 0;
+    uint32_t n = 0;
+    visit(s0, s1, [&](const float (&v)[4], Places at) {
+        bool stays[4], any = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            stays[e] = v[e] > -INFINITY && at_least(v[e], lo + at(e), cut);
+            any |= stays[e];
+        }
+        if (any) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const u64 x = weight(v[e]);
+                if (stays[e]) { w += x; ++n; }
+            }
+        }
+    });
     w = warp_total(w);
     n = warp_total(n);
     __syncthreads();
@@ -628,30 +782,44 @@ sample_filtered_kernel(const Args a) {
     const uint32_t his_n = lane < ranks ? cluster.map_shared_rank(&s, lane)->part_n : 0;
     const u64 whole = warp_total(his_w), before_cta = warp_total(lane < rank ? his_w : 0);
     const uint32_t kept = warp_total(his_n);
-    u64 before = before_cta + warp_total(lane < warp ? s.warp_w[lane] : 0);
     const u64 target = target_of(a.uniform[r], whole);
-    if (before <= target && target < before + w) {                 // (warp-uniform) this warp holds the pick
-        for (int i = s0 + lane; i - lane < s1; i += 32) {
-            u64 x = 0;
-            if (i < s1) {
-                const float v = value(i);
-                if (v > -INFINITY && entry(v, lo + i) >= cut) x = weight(v);
-            }
-            u64 incl = x;
+    const u64 cta_w = __shfl_sync(0xffffffffu, his_w, rank);
+    if (before_cta <= target && target < before_cta + cta_w) {     // (the whole CTA) the pick lies in this stretch
+        // the warp's part that holds it, cut into parts for all warps once more
+        u64 before = before_cta;
+        int part = 0;
+        while (part < WARPS - 1 && target >= before + s.warp_w[part]) before += s.warp_w[part++];
+        const int p0 = min(count, part * seg), p1 = min(count, p0 + seg), sub = ((seg + WARPS - 1) / WARPS + 7) / 8 * 8;
+        const int q0 = min(p1, p0 + warp * sub), q1 = min(p1, q0 + sub);
+        u64 x = 0;
+        visit(q0, q1, [&](const float (&v)[4], Places at) {
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const u64 up = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += up;
-            }
-            const unsigned past = __ballot_sync(0xffffffffu, before + incl > target);
-            if (past) {
-                if (lane == __ffs(past) - 1) {
-                    a.out[r] = lo + i;
-                    if (a.kept) a.kept[r] = (int)kept;
+            for (int e = 0; e < 4; ++e) x += kept_weight(v[e], at(e), cut);
+        });
+        x = warp_total(x);
+        __syncthreads();                                           // (the parts' sums have been read)
+        if (lane == 0) s.warp_w[warp] = x;
+        __syncthreads();
+        before += warp_total(lane < warp ? s.warp_w[lane] : 0);
+        if (before <= target && target < before + x) {             // (warp-uniform)
+            for (int i = q0 + lane; i - lane < q1; i += 32) {
+                const u64 mine = i < q1 ? kept_weight(value(i), i, cut) : 0;
+                u64 incl = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const u64 up = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += up;
                 }
-                break;
+                const unsigned past = __ballot_sync(0xffffffffu, before + incl > target);
+                if (past) {
+                    if (lane == __ffs(past) - 1) {
+                        a.out[r] = lo + i;
+                        if (a.kept) a.kept[r] = (int)kept;
+                    }
+                    break;
+                }
+                before += __shfl_sync(0xffffffffu, incl, 31);
             }
-            before += __shfl_sync(0xffffffffu, incl, 31);
         }
     }
     cluster.sync();
@@ -707,8 +875,10 @@ extern "C" int imparo_sample_filtered(const void* logits, int dtype, long long l
     sf::Args a;
     a.logits = logits; a.temperature = temperature; a.uniform = uniform; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p;
     a.out = out; a.kept = kept; a.ld = ld; a.vocab = vocab;
+    // As many CTAs per row as fill the chip about twice (two CTAs per SM), as long as each has 2,048 entries: a row's CTAs wait for one
+    // another a few times, so more of them pay only where SMs would have nothing to do or a long row would hold up the end.
     int ranks = 1;
-    while (ranks < 8 && vocab > 2048 * ranks) ranks <<= 1;
+    while (ranks < sf::MOST_RANKS && vocab > 2048 * ranks && (long long)n_rows * ranks < 592) ranks <<= 1;
     a.per = ((vocab + ranks - 1) / ranks + 7) / 8 * 8;
     // sums of vocab weights of at most 2^shift stay below 2^62
     a.shift = 62;
