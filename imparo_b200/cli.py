@@ -1,7 +1,7 @@
 """Command line, in the manner of the reference's token-id instrument and server flags:
 
     python -m imparo_b200 -m MODEL_DIR [--decode N] [--repeat N] [-c CTX] [-np PARALLEL]
-                          [--temperature T] [--seed S] [--dtype bfloat16|float32]
+                          [--temperature T] [--top-k K] [--top-p P] [--min-p P] [--seed S] [--dtype bfloat16|float32]
                           (TOKEN... | -t FILE | --prompt-len N [--batch B])
 
 Names and meanings follow the reference where it has them: `-m/--model`, `-c/--ctx`
@@ -9,7 +9,8 @@ Names and meanings follow the reference where it has them: `-m/--model`, `-c/--c
 (imparo-server/src/main.rs:178-240); `--decode N` (N new tokens after the prompt, the
 token trail is printed), `--repeat N`, token ids as arguments or `-t FILE`
 (imparo-model/src/bin/imparo-forward.rs:1036-1075,1343-1358).  The request fields
-max_tokens and temperature map to --decode and --temperature.  `--random CONFIG.json`
+max_tokens and temperature map to --decode and --temperature; --top-k, --top-p and --min-p
+filter the tokens a temperature samples from.  `--random CONFIG.json`
 draws random weights for a configuration instead of reading a model folder.
 """
 from __future__ import annotations
@@ -34,6 +35,9 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--decode", type=int, default=16, metavar="N", help="new tokens per request (the request's max_tokens)")
     ap.add_argument("--repeat", type=int, default=1, metavar="N", help="run the same requests N times (determinism check)")
     ap.add_argument("--temperature", type=float, default=0.0, help="0 is greedy")
+    ap.add_argument("--top-k", type=int, default=0, metavar="K", help="sample among the K most likely tokens (0: all)")
+    ap.add_argument("--top-p", type=float, default=1.0, metavar="P", help="of these, the fewest that reach probability P (1: all)")
+    ap.add_argument("--min-p", type=float, default=0.0, metavar="P", help="of these, the ones at least P times as likely as the most likely one")
     ap.add_argument("-t", "--tokens-file", metavar="FILE", help="token ids, whitespace-separated, one prompt per line")
     ap.add_argument("--prompt-len", type=int, help="uniform-random prompts of this length instead of given ids")
     ap.add_argument("--batch", type=int, default=1, help="with --prompt-len: how many prompts")
@@ -85,7 +89,8 @@ def main(argv=None) -> int:
     for rep in range(args.repeat):
         t1 = time.perf_counter()
         outs.append(engine.generate(prompts, max_tokens=args.decode, temperature=args.temperature,
-                                    seed=[args.seed + i for i in range(len(prompts))]))
+                                    seed=[args.seed + i for i in range(len(prompts))], top_k=args.top_k, top_p=args.top_p,
+                                    min_p=args.min_p))
         dt = time.perf_counter() - t1
         n_new = sum(len(o) for o in outs[-1])
         if not args.json:

@@ -33,6 +33,22 @@ from .step import StepFunction, StepItem, int_array
 _PRECISIONS = {"bfloat16": "bfloat16", "bf16": "bfloat16", "float32": "float32", "fp32": "float32", "f32": "float32"}
 
 
+def checked_filters(n: int, top_ks: Sequence[int], top_ps: Sequence[float], min_ps: Sequence[float]):
+    """The three filters of n requests, or none at all where no request has one."""
+    for name, values in (("top_k", top_ks), ("top_p", top_ps), ("min_p", min_ps)):
+        if len(values) != n:
+            raise ValueError(f"{name}: {len(values)} values for {n} prompts")
+    if any(int(k) != k or k < 0 for k in top_ks):
+        raise ValueError("top_k must be a whole number, 0 (all tokens) or more")
+    if not all(0 < p <= 1 for p in top_ps):
+        raise ValueError("top_p must be above 0 and at most 1 (all tokens)")
+    if not all(0 <= m <= 1 for m in min_ps):
+        raise ValueError("min_p must be from 0 (all tokens) to 1")
+    if any(k > 0 for k in top_ks) or any(p < 1 for p in top_ps) or any(m > 0 for m in min_ps):
+        return top_ks, top_ps, min_ps
+    return ()
+
+
 class Engine:
     def _model_spec(self, folder: Optional[str]):
         """The architecture's ModelSpec.  An architecture some of whose sizes only a tensor's shape gives takes the
@@ -184,21 +200,26 @@ class Engine:
     # -- generation --------------------------------------------------------------------------
     def generate(self, prompts: Sequence[Sequence[int]], max_tokens: Union[int, Sequence[int]] = 16,
                  temperature: Union[float, Sequence[float]] = 0.0, seed: Union[int, Sequence[int]] = 0,
-                 stop_token_ids: Optional[Sequence[int]] = None, on_step=None) -> List[List[int]]:
+                 stop_token_ids: Optional[Sequence[int]] = None, on_step=None, top_k: Union[int, Sequence[int]] = 0,
+                 top_p: Union[float, Sequence[float]] = 1.0, min_p: Union[float, Sequence[float]] = 0.0) -> List[List[int]]:
         """Continuous batching over the prompts (lists of token ids).  Returns the generated
         ids per prompt.  temperature 0 is greedy; seed keys the per-request random stream.
+        top_k, top_p and min_p filter the tokens a sampled request may take, in this order: the top_k most likely ones (0: all), of
+        these the fewest that reach top_p of their probability (1: all), of these the ones at least min_p times as likely as the
+        most likely one (0: all).  Each may be a list, one value per prompt.
         A stop token ends its request and is not part of the output.  A request that cannot
         fit the cache even alone ends with what it has (see failed in stats())."""
         previous = ops.use_state(self.rt.launch_state)       # the sampler's launches use this engine's scratch too
         try:
-            return self._generate(prompts, max_tokens, temperature, seed, stop_token_ids, on_step)
+            return self._generate(prompts, max_tokens, temperature, seed, stop_token_ids, on_step, top_k, top_p, min_p)
         finally:
             ops.use_state(previous)
 
-    def _generate(self, prompts, max_tokens, temperature, seed, stop_token_ids, on_step):
+    def _generate(self, prompts, max_tokens, temperature, seed, stop_token_ids, on_step, top_k=0, top_p=1.0, min_p=0.0):
         n = len(prompts)
         as_list = lambda v: list(v) if isinstance(v, (list, tuple)) else [v] * n
         max_new, temps, seeds = as_list(max_tokens), as_list(temperature), as_list(seed)
+        filters = checked_filters(n, as_list(top_k), as_list(top_p), as_list(min_p))
         stops = set(self.model.spec.eos_token_ids if stop_token_ids is None else stop_token_ids)
         sched = Scheduler(self.cache, self.max_step_tokens, self.parallel, self.ctx, count_padded_rows=self.step_fn.pad_rows)
         tokens: Dict[int, List[int]] = {}
@@ -295,7 +316,8 @@ class Engine:
             if all_wanting:
                 pending = self.sampler.sample_async(logits, [temps[index[e.request]] for e in all_wanting],
                                                     [seeds[index[e.request]] for e in all_wanting],
-                                                    [gen[e.request] for e in all_wanting])
+                                                    [gen[e.request] for e in all_wanting],
+                                                    *([values[index[e.request]] for e in all_wanting] for values in filters))
                 for e in wanting:
                     gen[e.request] += 1
                     sched.on_token(e.request, False)          # optimistic: a stop token is booked when it is read

@@ -6,11 +6,16 @@ temperature argument is ignored (imparo-server/src/main.rs:3383-3390).  Temperat
 sampling here: p = softmax(logits / T) in 32-bit, one uniform number u per (seed, step)
 from a counter-based generator, and the pick is the first index whose running sum of p
 in vocabulary order exceeds u * sum(p).  T == 0 is greedy.
+
+A request may also filter its tokens: top-k, then top-p of what that leaves, then min-p (ops.sample_filtered).  Its
+pick is made in sums that are exact for all practical purposes; requests without a filter are picked as above, whatever
+the others of the step ask for.
 """
 from __future__ import annotations
 
 from typing import List, Optional, Sequence
 
+import numpy as np
 import torch
 
 from ..kernels import ops
@@ -53,21 +58,28 @@ class Sampler:
         if n <= self._cap:
             return
         self._cap = n
-        self._host_in = [torch.empty((2, n), dtype=torch.float32, pin_memory=True) for _ in range(self.RING)]
-        self._dev_in = torch.empty((2, n), dtype=torch.float32, device=self.device)
+        # per row: temperature, uniform number; top_p, min_p, and as whole numbers top_k and whether the row filters
+        self._host_in = [torch.empty((6, n), dtype=torch.float32, pin_memory=True) for _ in range(self.RING)]
+        self._dev_in = torch.empty((6, n), dtype=torch.float32, device=self.device)
+        self._dev_filtered = torch.empty(n, dtype=torch.int32, device=self.device)
         self._dev_outs = [torch.empty(n, dtype=torch.int32, device=self.device) for _ in range(self.RING)]
         self._host_outs = [torch.empty(n, dtype=torch.int32, pin_memory=True) for _ in range(self.RING)]
 
     def sample(self, logits: torch.Tensor, temperatures: Optional[Sequence[float]] = None,
-               seeds: Optional[Sequence[int]] = None, steps: Optional[Sequence[int]] = None) -> List[int]:
+               seeds: Optional[Sequence[int]] = None, steps: Optional[Sequence[int]] = None,
+               top_ks: Optional[Sequence[int]] = None, top_ps: Optional[Sequence[float]] = None,
+               min_ps: Optional[Sequence[float]] = None) -> List[int]:
         """One token id per row of logits.  temperatures None or all 0: greedy.  Row r with
-        temperature > 0 uses uniform_for(seeds[r], steps[r]).  Reads the ids back (this is
+        temperature > 0 uses uniform_for(seeds[r], steps[r]).  top_ks, top_ps, min_ps: a filter per row each, or None
+        (0 or less, 1 or more, 0 or less: that row has none).  Reads the ids back (this is
         the step's device-to-host copy) and returns them as a list."""
-        return self.sample_async(logits, temperatures, seeds, steps).result()
+        return self.sample_async(logits, temperatures, seeds, steps, top_ks, top_ps, min_ps).result()
 
     def sample_async(self, logits: torch.Tensor, temperatures: Optional[Sequence[float]] = None,
-                     seeds: Optional[Sequence[int]] = None, steps: Optional[Sequence[int]] = None) -> PendingSample:
-        """Like sample(), without waiting: the kernel and the device-to-host copy are queued."""
+                     seeds: Optional[Sequence[int]] = None, steps: Optional[Sequence[int]] = None,
+                     top_ks: Optional[Sequence[int]] = None, top_ps: Optional[Sequence[float]] = None,
+                     min_ps: Optional[Sequence[float]] = None) -> PendingSample:
+        """Like sample(), without waiting: the kernels and the device-to-host copy are queued."""
         n = logits.shape[0]
         self._grow(n)
         self._turn = (self._turn + 1) % self.RING
@@ -77,12 +89,29 @@ class Sampler:
         else:
             h = self._host_in[self._turn]
             hn = h.numpy()                      # the same pinned memory: element writes without tensor indexing
+            filtered = 0
+            if top_ks is not None or top_ps is not None or min_ps is not None:
+                whole = hn.view(np.int32)
+                for r in range(n):
+                    k = min(int(top_ks[r]), 1 << 30) if top_ks is not None else 0
+                    p = float(top_ps[r]) if top_ps is not None else 1.0
+                    m = float(min_ps[r]) if min_ps is not None else 0.0
+                    hn[2, r], hn[3, r], whole[4, r] = p, m, max(k, 0)
+                    whole[5, r] = filters = temperatures[r] > 0 and (k > 0 or p < 1 or m > 0)
+                    filtered += filters
             for r in range(n):
                 t = float(temperatures[r])
                 hn[0, r] = t
                 hn[1, r] = uniform_for(seeds[r], steps[r]) if t > 0 else 0.0
-            self._dev_in[:, :n].copy_(h[:, :n], non_blocking=True)
-            ops.sample_rows(logits, self._dev_in[0, :n], self._dev_in[1, :n], out)
+            dev = self._dev_in[:6 if filtered else 2, :n]
+            dev.copy_(h[:6 if filtered else 2, :n], non_blocking=True)
+            if filtered < n:
+                ops.sample_rows(logits, dev[0], dev[1], out)
+            if filtered:
+                picked = out if filtered == n else self._dev_filtered[:n]
+                ops.sample_filtered(logits, dev[0], dev[1], picked, top_k=dev[4].view(torch.int32), top_p=dev[2], min_p=dev[3])
+                if picked is not out:
+                    torch.where(dev[5].view(torch.int32) != 0, picked, out, out=out)
         host = self._host_outs[self._turn][:n]
         host.copy_(out, non_blocking=True)
         ev = torch.cuda.Event()
