@@ -39,6 +39,16 @@ __device__ __forceinline__ int group_of(const Args& a, int t) {
     const int g = lo - 1;
     return g >= 0 && t < a.group_start[g + 1] ? g : -1;
 }
+// The group of one row for a whole CTA: with few groups every thread looks at one, which is one trip to memory instead of a search's.
+__device__ __forceinline__ int group_of_cta(const Args& a, int t, int* scratch) {
+    if (a.n_groups > (int)blockDim.x) return group_of(a, t);
+    if (threadIdx.x == 0) *scratch = -1;
+    __syncthreads();
+    const int g = threadIdx.x;
+    if (g < a.n_groups && a.group_start[g] <= t && t < a.group_start[g + 1]) *scratch = g;
+    __syncthreads();
+    return *scratch;
+}
 __device__ __forceinline__ const int* table_row(const Args& a, int t, int kernel) {
     const int item = a.item_of_token[t];
     if (item < 0 || item >= a.n_items) {

@@ -487,9 +487,10 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         // the results of the tiles with the same rows, for the first of them to add: [tile][dims, max, sum][row], where keys and values were
         float* other = reinterpret_cast<float*>(k_s);
         constexpr int OTHER = (HD + 2) * TILE;
-        static_assert((size_t)(NT - 1) * OTHER * 4 <= (size_t)ST * 2 * C::KEY_BYTES, "the results of the other tiles");
+        static_assert((size_t)(NT - 1) * OTHER * 4 <= (size_t)ST * 2 * C::KEY_BYTES && (size_t)NT / 2 * TILE * HD * 4 <= (size_t)NT * C::Q_BYTES &&
+                      (size_t)NT * TILE * HD * 4 <= (size_t)NT * C::Q_BYTES + (size_t)ST * 2 * C::KEY_BYTES, "results in shared memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(NT * 128) : "memory");                          // all tiles' products have run
         if (phases > 1) {
-            asm volatile("bar.sync 1, %0;" ::"n"(NT * 128) : "memory");                      // all tiles' products have run
             if (x >= R && ok) {
                 float* mine = other + (x - R) * OTHER + r;
                 if (n_x > 0 && warp_valid) {
@@ -525,6 +526,9 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                     }
                 }
             }
+            // by way of shared memory (where the queries were, and with four tiles of rows the keys): a thread has a row, which alone
+            // it would write 16 bytes at a time, far from its neighbours'
+            float4* rows = reinterpret_cast<float4*>(q_s) + (size_t)(x * TILE + (warp & 3) * 32) * (HD / 4);
 #pragma unroll 1
             for (int c = 0; c < HD; c += 16) {
                 float o[16];
@@ -537,11 +541,16 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll
                         for (int e = 0; e < 16; ++e) o[e] += other[(x + (i - 1) * R) * OTHER + (c + e) * TILE + r] * f[i];
                     }
-                if (valid) {
-                    float4* dst = reinterpret_cast<float4*>(a.part_acc + part * HD + c);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-                }
+                for (int e = 0; e < 4; ++e)
+                    rows[lane * (HD / 4) + ((c / 4 + e) ^ (lane & 7))] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            }
+            __syncwarp();
+            constexpr int LANES = HD / 4;                    // 16 bytes each to a row
+            for (int i = lane / LANES; i < 32; i += 32 / LANES) {
+                const size_t his = __shfl_sync(0xffffffffu, part, i);
+                if ((warp & 3) * 32 + i < toks * G)
+                    reinterpret_cast<float4*>(a.part_acc)[his * (HD / 4) + lane % LANES] = rows[i * (HD / 4) + ((lane % LANES) ^ (i & 7))];
             }
             if (valid) {
                 const bool sees = a.positions[t] >= 0;       // (a row without a position sees nothing)
@@ -569,41 +578,48 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <int HD, bool JOIN>
-__global__ void __launch_bounds__(OWN_WARPS * 32)
+// WIDE: up to 16 heads; otherwise at most eight, the lower half of the tile stays empty and costs no registers.
+template <int HD, bool JOIN, bool WIDE>
+__global__ void __launch_bounds__(OWN_WARPS * 32, HD == 64 ? (WIDE ? 4 : 5) : (WIDE ? 2 : 3))
 own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __restrict__ sinks, const int n_splits) {
     constexpr int NB = HD / 64, KB = HD / 32;                // 64-dim blocks (values), 32-dim blocks (keys)
-    __shared__ int span_scratch[2];
-    __shared__ float w_m[OWN_WARPS][16], w_l[OWN_WARPS][16];
-    __shared__ __align__(16) float w_o[OWN_WARPS][16][HD + 4];
+    __shared__ int span_scratch[3];
+    constexpr int HEADS = WIDE ? 16 : 8;
+    __shared__ float w_m[OWN_WARPS][HEADS], w_l[OWN_WARPS][HEADS];
+    __shared__ __align__(16) float w_o[OWN_WARPS][HEADS][HD + 4];
     pdl_trigger();
     pdl_no_wait();                                           // (what this reads before its wait was complete before the kernel ahead let it start)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tg = lane & 3;
     const int G = a.nh / a.nkv, head_tiles = (G + 15) / 16;
     const int kvh = blockIdx.x / head_tiles, head0 = kvh * G + blockIdx.x % head_tiles * 16, n_heads = min(16, kvh * G + G - head0);
     const int t = blockIdx.y, split = blockIdx.z;
-    const int group = group_of(a, t);
+    const int pos = a.positions[t], item = a.item_of_token[t];           // (on their way while the group is found)
+    const int group = group_of_cta(a, t, span_scratch + 2);
     const Span span = shared_span(a, group, span_scratch);
-    const Own own = own_keys(a, a.positions[t], span);
+    const Own own = own_keys(a, pos, span);
     const int k0 = (int)min((long long)split * a.chunk_own, (long long)own.count);
     const int k1 = split + 1 == a.n_own ? own.count : (int)min((long long)k0 + a.chunk_own, (long long)own.count);
-    const int* tab = k0 < k1 ? table_row(a, t, 84) : nullptr;
+    if (k0 < k1 && (item < 0 || item >= a.n_items) && tid == 0) report(a.status, IMPARO_ST_PAGE_RANGE, 84, t, item);
+    const int* tab = k0 < k1 && item >= 0 && item < a.n_items ? a.table + (size_t)item * a.max_blocks : nullptr;
     const size_t kvw = (size_t)a.nkv * HD;
     const __nv_bfloat16* kc = reinterpret_cast<const __nv_bfloat16*>(a.k) + (size_t)kvh * HD;
     const __nv_bfloat16* vc = reinterpret_cast<const __nv_bfloat16*>(a.v) + (size_t)kvh * HD;
     // the queries: heads g and g + 8, dims 32 b + 8 tg .. + 7
-    uint4 qa[KB], qb[KB];
+    uint4 qa[KB], qb[WIDE ? KB : 1];
+    if (!WIDE) qb[0] = make_uint4(0u, 0u, 0u, 0u);
     {
         const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)t * a.q_stride + (size_t)head0 * HD + tg * 8;
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
             qa[b] = g < n_heads ? *reinterpret_cast<const uint4*>(q + (size_t)g * HD + b * 32) : make_uint4(0u, 0u, 0u, 0u);
-            qb[b] = g + 8 < n_heads ? *reinterpret_cast<const uint4*>(q + (size_t)(g + 8) * HD + b * 32) : make_uint4(0u, 0u, 0u, 0u);
+            if (WIDE) qb[b] = g + 8 < n_heads ? *reinterpret_cast<const uint4*>(q + (size_t)(g + 8) * HD + b * 32) : make_uint4(0u, 0u, 0u, 0u);
         }
     }
-    float o[NB * 8][4];                                      // output tile nb * 8 + i: dims 64 nb + 8 column + i
+    float o[NB * 8][WIDE ? 4 : 2];                           // output tile nb * 8 + i: dims 64 nb + 8 column + i
 #pragma unroll
-    for (int i = 0; i < NB * 8; ++i) { o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f; }
+    for (int i = 0; i < NB * 8; ++i)
+#pragma unroll
+        for (int e = 0; e < (WIDE ? 4 : 2); ++e) o[i][e] = 0.f;
     float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.f, l_b = 0.f;
     const float sl2 = a.scale * LOG2E;
     if (tab != nullptr) {
@@ -638,8 +654,9 @@ own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __rest
                 s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
                 for (int b = 0; b < KB; ++b) {
-                    mma16816(s[n], qa[b].x, qb[b].x, qa[b].y, qb[b].y, kf[n][b].x, kf[n][b].y);
-                    mma16816(s[n], qa[b].z, qb[b].z, qa[b].w, qb[b].w, kf[n][b].z, kf[n][b].w);
+                    const uint4 q2 = qb[WIDE ? b : 0];
+                    mma16816(s[n], qa[b].x, q2.x, qa[b].y, q2.y, kf[n][b].x, kf[n][b].y);
+                    mma16816(s[n], qa[b].z, q2.z, qa[b].w, q2.w, kf[n][b].z, kf[n][b].w);
                 }
             }
             float mx_a = -INFINITY, mx_b = -INFINITY;
@@ -674,7 +691,11 @@ own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __rest
                     l_b += s[n][2 + e];
                 }
 #pragma unroll
-            for (int i = 0; i < NB * 8; ++i) { o[i][0] *= ca; o[i][1] *= ca; o[i][2] *= cb; o[i][3] *= cb; }
+            for (int i = 0; i < NB * 8; ++i) {
+                o[i][0] *= ca;
+                o[i][1] *= ca;
+                if (WIDE) { o[i][WIDE ? 2 : 0] *= cb; o[i][WIDE ? 3 : 1] *= cb; }
+            }
             const uint32_t p0 = pack_bf16(s[0][0], s[0][1]), p1 = pack_bf16(s[0][2], s[0][3]), p2 = pack_bf16(s[1][0], s[1][1]),
                            p3 = pack_bf16(s[1][2], s[1][3]);
 #pragma unroll
@@ -684,7 +705,12 @@ own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __rest
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const uint32_t pick = i & 1 ? 0x7632u : 0x5410u;
-                    mma16816(o[b * 8 + i], p0, p1, p2, p3, __byte_perm(x0[i >> 1], x1[i >> 1], pick), __byte_perm(x2[i >> 1], x3[i >> 1], pick));
+                    float (&acc)[WIDE ? 4 : 2] = o[b * 8 + i];
+                    float c[4] = {acc[0], acc[1], WIDE ? acc[WIDE ? 2 : 0] : 0.f, WIDE ? acc[WIDE ? 3 : 1] : 0.f};
+                    mma16816(c, p0, WIDE ? p1 : 0u, p2, WIDE ? p3 : 0u, __byte_perm(x0[i >> 1], x1[i >> 1], pick), __byte_perm(x2[i >> 1], x3[i >> 1], pick));
+                    acc[0] = c[0];
+                    acc[1] = c[1];
+                    if (WIDE) { acc[WIDE ? 2 : 0] = c[2]; acc[WIDE ? 3 : 1] = c[3]; }
                 }
             }
         }
@@ -693,7 +719,8 @@ own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __rest
         l_b += __shfl_xor_sync(0xffffffffu, l_b, 1);
         l_b += __shfl_xor_sync(0xffffffffu, l_b, 2);
     }
-    if (tg == 0) { w_m[warp][g] = m_a; w_l[warp][g] = l_a; w_m[warp][g + 8] = m_b; w_l[warp][g + 8] = l_b; }
+    if (tg == 0) { w_m[warp][g] = m_a; w_l[warp][g] = l_a; }
+    if (WIDE && tg == 0) { w_m[warp][g + 8] = m_b; w_l[warp][g + 8] = l_b; }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         // a lane's columns of the eight tiles are 2 tg and 2 tg + 1: dims 8 (2 tg) .. + 7 and the eight behind them
@@ -703,9 +730,12 @@ own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __rest
             for (int h = 0; h < 2; ++h) {
                 float* dst = &w_o[warp][g][b * 64 + 8 * (2 * tg + e) + 4 * h];
                 *reinterpret_cast<float4*>(dst) = make_float4(o[b * 8 + 4 * h][e], o[b * 8 + 4 * h + 1][e], o[b * 8 + 4 * h + 2][e], o[b * 8 + 4 * h + 3][e]);
-                dst = &w_o[warp][g + 8][b * 64 + 8 * (2 * tg + e) + 4 * h];
-                *reinterpret_cast<float4*>(dst) = make_float4(o[b * 8 + 4 * h][2 + e], o[b * 8 + 4 * h + 1][2 + e], o[b * 8 + 4 * h + 2][2 + e],
-                                                              o[b * 8 + 4 * h + 3][2 + e]);
+                if (WIDE) {
+                    constexpr int LOW = WIDE ? 2 : 0;
+                    dst = &w_o[warp][WIDE ? g + 8 : 0][b * 64 + 8 * (2 * tg + e) + 4 * h];
+                    *reinterpret_cast<float4*>(dst) = make_float4(o[b * 8 + 4 * h][LOW + e], o[b * 8 + 4 * h + 1][LOW + e],
+                                                                  o[b * 8 + 4 * h + 2][LOW + e], o[b * 8 + 4 * h + 3][LOW + e]);
+                }
             }
         }
     }
@@ -834,8 +864,9 @@ static int launch_hd(const Args& a, __nv_bfloat16* out, const float* sinks, cuda
     e = launch(shared_tc_kernel<HD>, dim3(a.nkv, a.n_shared, (unsigned)units), dim3(Shape<HD>::THREADS), Shape<HD>::SMEM, stream, mk, mv, a, n_splits);
     if (e != cudaSuccess) return (int)e;
     const dim3 grid(a.nkv * head_tiles, a.n_rows, a.n_own);
-    e = a.n_own == 1 ? launch(own_tc_kernel<HD, true>, grid, dim3(OWN_WARPS * 32), 0, stream, a, out, sinks, n_splits)
-                     : launch(own_tc_kernel<HD, false>, grid, dim3(OWN_WARPS * 32), 0, stream, a, out, sinks, n_splits);
+    auto own = G > 8 ? (a.n_own == 1 ? own_tc_kernel<HD, true, true> : own_tc_kernel<HD, false, true>)
+                     : (a.n_own == 1 ? own_tc_kernel<HD, true, false> : own_tc_kernel<HD, false, false>);
+    e = launch(own, grid, dim3(OWN_WARPS * 32), 0, stream, a, out, sinks, n_splits);
     return e == cudaSuccess ? 0 : (int)e;
 }
 
