@@ -16,13 +16,25 @@ namespace sp {
 
 // ---- any head size, 32-bit or bfloat16 -------------------------------------------------------------------------------
 // A CTA takes up to 16 rows (tokens of one group x query heads of one kv head) and one stretch of keys, 32 keys at a time in shared
-// memory; eight threads per row make four scores each, then an eighth of the row's output each.
+// memory; eight threads per row make four scores each, then an eighth of the row's output each.  What bounds it is the chain of a
+// stretch's few tiles (page lookup, keys and values, scores, weights): short stretches on many CTAs, up to four per SM.
 constexpr int ROWS = 16, KEYS = 32, THREADS = 128;
 constexpr int MOST_HEAD = 256;
 
-template <typename T>
+// 16 bytes of a cache row as 32-bit numbers
+__device__ __forceinline__ void unpack16(const uint4& x, const float*, float (&v)[4]) {
+    v[0] = __uint_as_float(x.x); v[1] = __uint_as_float(x.y); v[2] = __uint_as_float(x.z); v[3] = __uint_as_float(x.w);
+}
+__device__ __forceinline__ void unpack16(const uint4& x, const __nv_bfloat16*, float (&v)[8]) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+
+// HM: the head size rounded up to 64, 128 or 256.  aligned: the caches start on 16 bytes (their rows then do too).
+template <typename T, int HM>
 __global__ void __launch_bounds__(THREADS)
-shared_any_kernel(const Args a) {
+shared_any_kernel(const Args a, const int aligned) {
     extern __shared__ __align__(16) float sp_smem[];
     __shared__ int key_row[KEYS], span_scratch[2];
     const int hd = a.hd, ks_stride = hd + 4;
@@ -91,14 +103,15 @@ shared_any_kernel(const Args a) {
     const T* q = reinterpret_cast<const T*>(a.q);
     const T* kc = reinterpret_cast<const T*>(a.k) + (size_t)kvh * hd;
     const T* vc = reinterpret_cast<const T*>(a.v) + (size_t)kvh * hd;
-    for (int i = tid; i < n_rows * hd; i += THREADS) {
-        const int rr = i / hd;
-        qs[i] = to_f32(q[(size_t)(row0 + rr / n_heads) * a.q_stride + (size_t)(kvh * G + head0 + rr % n_heads) * hd + i % hd]);
+    // (eight threads a row in every loop: no division by the head size)
+    if (written) {
+        const T* src = q + (size_t)t * a.q_stride + (size_t)head * hd;
+        for (int d = sub; d < hd; d += 8) qs[r * hd + d] = to_f32(src[d]);
     }
-    constexpr int OUT = MOST_HEAD / 8;                             // outputs of a thread: dims sub, sub + 8, ...
-    float o[OUT];
+    constexpr int OUT = HM / 32, VEC = 16 / sizeof(T);             // outputs of a thread: four dims from 4 sub on, every 32
+    float4 o[OUT];
 #pragma unroll
-    for (int i = 0; i < OUT; ++i) o[i] = 0.f;
+    for (int i = 0; i < OUT; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     float m = -INFINITY, l = 0.f;
     for (int key0 = k0; tab != nullptr && key0 < k1; key0 += KEYS) {
         const int n = min(KEYS, k1 - key0);
@@ -114,11 +127,42 @@ shared_any_kernel(const Args a) {
             key_row[tid] = at_row;
         }
         __syncthreads();
-#pragma unroll 4
-        for (int i = tid; i < KEYS * hd; i += THREADS) {
-            const int j = i / hd, d = i % hd, at_row = key_row[j];
-            ks[j * ks_stride + d] = at_row >= 0 ? to_f32(kc[(size_t)at_row * kvw + d]) : 0.f;
-            vs[i] = at_row >= 0 ? to_f32(vc[(size_t)at_row * kvw + d]) : 0.f;
+        if (aligned) {
+            // both tiles' loads of a thread are on their way before the first is used
+            constexpr int TURNS = KEYS / ROWS, MOST = HM / VEC / 8 > 0 ? HM / VEC / 8 : 1;
+#pragma unroll
+            for (int c = 0; c < MOST; ++c) {
+                const int at = (sub + 8 * c) * VEC;
+                uint4 x[TURNS][2];
+#pragma unroll
+                for (int u = 0; u < TURNS; ++u) {
+                    const int at_row = key_row[r + u * ROWS];
+                    const bool there = at_row >= 0 && at < hd;
+                    x[u][0] = there ? *reinterpret_cast<const uint4*>(kc + (size_t)at_row * kvw + at) : make_uint4(0u, 0u, 0u, 0u);
+                    x[u][1] = there ? *reinterpret_cast<const uint4*>(vc + (size_t)at_row * kvw + at) : make_uint4(0u, 0u, 0u, 0u);
+                }
+                if (at < hd) {
+#pragma unroll
+                    for (int u = 0; u < TURNS; ++u) {
+                        const int j = r + u * ROWS;
+                        float v[VEC];
+                        unpack16(x[u][0], kc, v);
+#pragma unroll
+                        for (int e = 0; e < VEC; e += 4) *reinterpret_cast<float4*>(ks + j * ks_stride + at + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                        unpack16(x[u][1], vc, v);
+#pragma unroll
+                        for (int e = 0; e < VEC; e += 4) *reinterpret_cast<float4*>(vs + j * hd + at + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                    }
+                }
+            }
+        } else {
+            for (int j = r; j < KEYS; j += ROWS) {
+                const int at_row = key_row[j];
+                for (int d = sub; d < hd; d += 8) {
+                    ks[j * ks_stride + d] = at_row >= 0 ? to_f32(kc[(size_t)at_row * kvw + d]) : 0.f;
+                    vs[j * hd + d] = at_row >= 0 ? to_f32(vc[(size_t)at_row * kvw + d]) : 0.f;
+                }
+            }
         }
         __syncthreads();
         float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -156,12 +200,17 @@ shared_any_kernel(const Args a) {
         m = m_new;
         __syncwarp();                                              // a row's probabilities are written and read by one warp
 #pragma unroll
-        for (int i = 0; i < OUT; ++i) o[i] *= corr;
+        for (int i = 0; i < OUT; ++i) { o[i].x *= corr; o[i].y *= corr; o[i].z *= corr; o[i].w *= corr; }
+#pragma unroll 4
         for (int j = 0; j < n; ++j) {
             const float p = ps[r * (KEYS + 1) + j];
 #pragma unroll
-            for (int i = 0; i < OUT; ++i)
-                if (sub + 8 * i < hd) o[i] += p * vs[j * hd + sub + 8 * i];
+            for (int i = 0; i < OUT; ++i) {
+                if (4 * sub + 32 * i < hd) {
+                    const float4 x = *reinterpret_cast<const float4*>(vs + j * hd + 4 * sub + 32 * i);
+                    o[i].x += p * x.x; o[i].y += p * x.y; o[i].z += p * x.z; o[i].w += p * x.w;
+                }
+            }
         }
     }
     if (written) {
@@ -170,7 +219,10 @@ shared_any_kernel(const Args a) {
         if (l > 0.f) {
 #pragma unroll
             for (int i = 0; i < OUT; ++i)
-                if (sub + 8 * i < hd) a.part_acc[at_part * hd + sub + 8 * i] = o[i];
+                if (4 * sub + 32 * i < hd) {
+                    float* dst = a.part_acc + at_part * hd + 4 * sub + 32 * i;       // (the scratch may start anywhere)
+                    dst[0] = o[i].x; dst[1] = o[i].y; dst[2] = o[i].z; dst[3] = o[i].w;
+                }
         }
     }
 }
@@ -182,12 +234,13 @@ static int launch_any(const Args& a, cudaStream_t stream) {
     const long long units = (tiles > a.n_rows ? tiles : a.n_rows) * head_tiles;
     if (units > 65535 || a.nkv > 65535) return -2;
     const size_t smem = sizeof(float) * (ROWS * a.hd + KEYS * (a.hd + 4) + KEYS * a.hd + ROWS * (KEYS + 1));
-    auto kern = shared_any_kernel<T>;
+    auto kern = a.hd <= 64 ? shared_any_kernel<T, 64> : a.hd <= 128 ? shared_any_kernel<T, 128> : shared_any_kernel<T, 256>;
     if (smem > 48 * 1024) {
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return (int)e;
     }
-    cudaError_t e = launch(kern, dim3(a.n_shared + a.n_own, a.nkv, (unsigned)units), dim3(THREADS), smem, stream, a);
+    const int aligned = (((uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0;
+    cudaError_t e = launch(kern, dim3(a.n_shared + a.n_own, a.nkv, (unsigned)units), dim3(THREADS), smem, stream, a, aligned);
     return e == cudaSuccess ? 0 : (int)e;
 }
 

@@ -70,24 +70,6 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// 2^x for two numbers x <= 8 on the multiply-add units, which have time where the exponential units have none: 2^x = 2^n 2^f, n whole,
-// |f| <= 1/2, and the cubic for 2^f whose largest relative error on that range is the least a cubic can have (7.5e-5, a fortieth of
-// the step of the bfloat16 that takes the result).  Adding 1.5 2^23 rounds to a whole number, which then lies in the low bits.
-__device__ __forceinline__ float2 exp2_fma(float2 x) {
-    const float2 whole = make_float2(12582912.f, 12582912.f);
-    x.x = fmaxf(x.x, -126.f);
-    x.y = fmaxf(x.y, -126.f);
-    const float2 n = __fadd2_rn(x, whole);
-    const float2 f = __fadd2_rn(x, __fadd2_rn(whole, make_float2(-n.x, -n.y)));
-    float2 p = __ffma2_rn(f, make_float2(0.05517165735f, 0.05517165735f), make_float2(0.24261112511f, 0.24261112511f));
-    p = __ffma2_rn(f, p, make_float2(0.69326096773f, 0.69326096773f));
-    p = __ffma2_rn(f, p, make_float2(0.99992805719f, 0.99992805719f));
-    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(n.x) << 23)),
-                       __int_as_float(__float_as_int(p.y) + (__float_as_int(n.y) << 23)));
-}
-#ifndef SP_FMA
-#define SP_FMA 0
-#endif
 // the largest of three; no number if one of them is none
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
@@ -463,8 +445,8 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         float2 e = __ffma2_rn(make_float2(sv[c * 32 + 2 * i], sv[c * 32 + 2 * i + 1]), sl, base);
-                        if (i * SP_FMA % 16 + SP_FMA >= 16) e = exp2_fma(e);
-                        else { e.x = ex2(e.x); e.y = ex2(e.y); }
+                        e.x = ex2(e.x);
+                        e.y = ex2(e.y);
                         sum[i & 1] = __fadd2_rn(sum[i & 1], e);
                         p[i] = pack_bf16(e.x, e.y);
                     }
@@ -565,7 +547,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 }
 
 // ---- a row's own keys, and the join ----------------------------------------------------------------------------------
-// One CTA per (stretch of own keys, kv head x tile of 16 query heads, token).  A warp takes 16 keys at a time on mma.sync: the heads
+// One CTA per (stretch of own keys, kv head x tile of 16 query heads, token).  A warp takes 16 or 32 keys at a time on mma.sync: the heads
 // are the rows of the tile, keys and values go from the cache to registers as 16-byte loads, whole 64- or 128-byte stretches of a
 // row at a time.  The products' inner index may run in any order that both operands share, and so may the outer one of P V: a lane's
 // eight neighbouring dims are four steps' fragments of the first product and its own column of eight output tiles of the second
@@ -580,11 +562,11 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
 
 // WIDE: up to 16 heads; otherwise at most eight, the lower half of the tile stays empty and costs no registers.
 template <int HD, bool JOIN, bool WIDE>
-__global__ void __launch_bounds__(OWN_WARPS * 32, HD == 64 ? (WIDE ? 4 : 5) : (WIDE ? 2 : 3))
+__global__ void __launch_bounds__(OWN_WARPS * 32, HD == 64 ? 4 : (WIDE ? 2 : 3))
 own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __restrict__ sinks, const int n_splits) {
     constexpr int NB = HD / 64, KB = HD / 32;                // 64-dim blocks (values), 32-dim blocks (keys)
     __shared__ int span_scratch[3];
-    constexpr int HEADS = WIDE ? 16 : 8;
+    constexpr int HEADS = WIDE ? 16 : 8, SLABS = HD == 64 && !WIDE ? 2 : 1;      // 16 keys each, all loads of a turn at once
     __shared__ float w_m[OWN_WARPS][HEADS], w_l[OWN_WARPS][HEADS];
     __shared__ __align__(16) float w_o[OWN_WARPS][HEADS][HD + 4];
     pdl_trigger();
@@ -623,31 +605,36 @@ own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __rest
     float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.f, l_b = 0.f;
     const float sl2 = a.scale * LOG2E;
     if (tab != nullptr) {
-        for (int base = k0 + warp * 16; base < k1; base += OWN_WARPS * 16) {
-            int row = -1;                                    // lane i < 16: where key base + i lies
-            if (lane < 16 && base + lane < k1) {
+        for (int base = k0 + warp * 16 * SLABS; base < k1; base += OWN_WARPS * 16 * SLABS) {
+            int row = -1;                                    // lane i: where key base + i lies
+            if (lane < 16 * SLABS && base + lane < k1) {
                 const int key = own.key(base + lane), block = key / a.page_size;
                 const int page = block < a.max_blocks ? tab[block] : -1;
                 if (page < 0 || page >= a.n_pages) report(a.status, IMPARO_ST_PAGE_RANGE, 85, t, page);
                 else row = page * a.page_size + key % a.page_size;
             }
             const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-            uint4 kf[2][KB], vf[4][NB];
+            uint4 kf[SLABS][2][KB], vf[SLABS][4][NB];
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const int at = __shfl_sync(0xffffffffu, row, n * 8 + g);
+            for (int slab = 0; slab < SLABS; ++slab) {
 #pragma unroll
-                for (int b = 0; b < KB; ++b)
-                    kf[n][b] = at >= 0 ? __ldg(reinterpret_cast<const uint4*>(kc + (size_t)at * kvw + b * 32 + tg * 8)) : zero;
-            }
+                for (int n = 0; n < 2; ++n) {
+                    const int at = __shfl_sync(0xffffffffu, row, slab * 16 + n * 8 + g);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {                    // keys 2 tg, 2 tg + 1, 2 tg + 8, 2 tg + 9
-                const int at = __shfl_sync(0xffffffffu, row, 2 * tg + (u & 1) + (u >> 1) * 8);
+                    for (int b = 0; b < KB; ++b)
+                        kf[slab][n][b] = at >= 0 ? __ldg(reinterpret_cast<const uint4*>(kc + (size_t)at * kvw + b * 32 + tg * 8)) : zero;
+                }
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
-                    vf[u][b] = at >= 0 ? __ldg(reinterpret_cast<const uint4*>(vc + (size_t)at * kvw + b * 64 + g * 8)) : zero;
+                for (int u = 0; u < 4; ++u) {                // keys 2 tg, 2 tg + 1, 2 tg + 8, 2 tg + 9
+                    const int at = __shfl_sync(0xffffffffu, row, slab * 16 + 2 * tg + (u & 1) + (u >> 1) * 8);
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+                        vf[slab][u][b] = at >= 0 ? __ldg(reinterpret_cast<const uint4*>(vc + (size_t)at * kvw + b * 64 + g * 8)) : zero;
+                }
             }
             const unsigned there = __ballot_sync(0xffffffffu, row >= 0);
+#pragma unroll
+            for (int slab = 0; slab < SLABS; ++slab) {
             float s[2][4];
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
@@ -655,8 +642,8 @@ own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __rest
 #pragma unroll
                 for (int b = 0; b < KB; ++b) {
                     const uint4 q2 = qb[WIDE ? b : 0];
-                    mma16816(s[n], qa[b].x, q2.x, qa[b].y, q2.y, kf[n][b].x, kf[n][b].y);
-                    mma16816(s[n], qa[b].z, q2.z, qa[b].w, q2.w, kf[n][b].z, kf[n][b].w);
+                    mma16816(s[n], qa[b].x, q2.x, qa[b].y, q2.y, kf[slab][n][b].x, kf[slab][n][b].y);
+                    mma16816(s[n], qa[b].z, q2.z, qa[b].w, q2.w, kf[slab][n][b].z, kf[slab][n][b].w);
                 }
             }
             float mx_a = -INFINITY, mx_b = -INFINITY;
@@ -664,7 +651,7 @@ own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __rest
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const bool seen = (there >> (n * 8 + 2 * tg + e)) & 1u;
+                    const bool seen = (there >> (slab * 16 + n * 8 + 2 * tg + e)) & 1u;
                     s[n][e] = seen ? s[n][e] * sl2 : -INFINITY;
                     s[n][2 + e] = seen ? s[n][2 + e] * sl2 : -INFINITY;
                     mx_a = fmaxf(mx_a, s[n][e]);
@@ -700,8 +687,8 @@ own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __rest
                            p3 = pack_bf16(s[1][2], s[1][3]);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const uint32_t x0[4] = {vf[0][b].x, vf[0][b].y, vf[0][b].z, vf[0][b].w}, x1[4] = {vf[1][b].x, vf[1][b].y, vf[1][b].z, vf[1][b].w};
-                const uint32_t x2[4] = {vf[2][b].x, vf[2][b].y, vf[2][b].z, vf[2][b].w}, x3[4] = {vf[3][b].x, vf[3][b].y, vf[3][b].z, vf[3][b].w};
+                const uint32_t x0[4] = {vf[slab][0][b].x, vf[slab][0][b].y, vf[slab][0][b].z, vf[slab][0][b].w}, x1[4] = {vf[slab][1][b].x, vf[slab][1][b].y, vf[slab][1][b].z, vf[slab][1][b].w};
+                const uint32_t x2[4] = {vf[slab][2][b].x, vf[slab][2][b].y, vf[slab][2][b].z, vf[slab][2][b].w}, x3[4] = {vf[slab][3][b].x, vf[slab][3][b].y, vf[slab][3][b].z, vf[slab][3][b].w};
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const uint32_t pick = i & 1 ? 0x7632u : 0x5410u;
@@ -712,6 +699,7 @@ own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __rest
                     acc[1] = c[1];
                     if (WIDE) { acc[WIDE ? 2 : 0] = c[2]; acc[WIDE ? 3 : 1] = c[3]; }
                 }
+            }
             }
         }
         l_a += __shfl_xor_sync(0xffffffffu, l_a, 1);
