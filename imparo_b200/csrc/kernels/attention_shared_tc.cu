@@ -605,15 +605,17 @@ own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __rest
     float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.f, l_b = 0.f;
     const float sl2 = a.scale * LOG2E;
     if (tab != nullptr) {
+        auto look_up = [&](int base) -> int {                // lane i: where key base + i lies
+            if (lane >= 16 * SLABS || base + lane >= k1) return -1;
+            const int key = own.key(base + lane), block = key / a.page_size;
+            const int page = block < a.max_blocks ? tab[block] : -1;
+            if (page >= 0 && page < a.n_pages) return page * a.page_size + key % a.page_size;
+            report(a.status, IMPARO_ST_PAGE_RANGE, 85, t, page);
+            return -1;
+        };
+        int next_row = look_up(k0 + warp * 16 * SLABS);
         for (int base = k0 + warp * 16 * SLABS; base < k1; base += OWN_WARPS * 16 * SLABS) {
-            int row = -1;                                    // lane i: where key base + i lies
-            if (lane < 16 * SLABS && base + lane < k1) {
-                const int key = own.key(base + lane), block = key / a.page_size;
-                const int page = block < a.max_blocks ? tab[block] : -1;
-                if (page < 0 || page >= a.n_pages) report(a.status, IMPARO_ST_PAGE_RANGE, 85, t, page);
-                else row = page * a.page_size + key % a.page_size;
-            }
-            const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+            const int row = next_row;
             uint4 kf[SLABS][2][KB], vf[SLABS][4][NB];
 #pragma unroll
             for (int slab = 0; slab < SLABS; ++slab) {
@@ -622,17 +624,29 @@ own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __rest
                     const int at = __shfl_sync(0xffffffffu, row, slab * 16 + n * 8 + g);
 #pragma unroll
                     for (int b = 0; b < KB; ++b)
-                        kf[slab][n][b] = at >= 0 ? __ldg(reinterpret_cast<const uint4*>(kc + (size_t)at * kvw + b * 32 + tg * 8)) : zero;
+                        kf[slab][n][b] = __ldg(reinterpret_cast<const uint4*>(kc + (size_t)max(at, 0) * kvw + b * 32 + tg * 8));
                 }
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {                // keys 2 tg, 2 tg + 1, 2 tg + 8, 2 tg + 9
                     const int at = __shfl_sync(0xffffffffu, row, slab * 16 + 2 * tg + (u & 1) + (u >> 1) * 8);
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
-                        vf[slab][u][b] = at >= 0 ? __ldg(reinterpret_cast<const uint4*>(vc + (size_t)at * kvw + b * 64 + g * 8)) : zero;
+                        vf[slab][u][b] = __ldg(reinterpret_cast<const uint4*>(vc + (size_t)max(at, 0) * kvw + b * 64 + g * 8));
                 }
             }
+            next_row = look_up(base + OWN_WARPS * 16 * SLABS);            // (a turn ahead: its keys need not wait for the table)
             const unsigned there = __ballot_sync(0xffffffffu, row >= 0);
+            // (places without a key read the cache's first row: their scores are left out, their values must be finite)
+            if (there != (SLABS == 2 ? 0xffffffffu : 0xffffu)) {
+#pragma unroll
+                for (int slab = 0; slab < SLABS; ++slab)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (!((there >> (slab * 16 + 2 * tg + (u & 1) + (u >> 1) * 8)) & 1u)) {
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) vf[slab][u][b] = make_uint4(0u, 0u, 0u, 0u);
+                        }
+            }
 #pragma unroll
             for (int slab = 0; slab < SLABS; ++slab) {
             float s[2][4];
