@@ -36,7 +36,7 @@ template <typename T, int HM>
 __global__ void __launch_bounds__(THREADS)
 shared_any_kernel(const Args a, const int aligned) {
     extern __shared__ __align__(16) float sp_smem[];
-    __shared__ int key_row[KEYS], span_scratch[2];
+    __shared__ int key_row[KEYS];
     const int hd = a.hd, ks_stride = hd + 4;
     float* qs = sp_smem;                                           // [ROWS][hd]
     float* ks = qs + ROWS * hd;                                    // [KEYS][hd + 4]
@@ -57,7 +57,7 @@ shared_any_kernel(const Args a, const int aligned) {
         row0 = unit;
         n_tok = 1;
         tab_of = row0;
-        group = group_of(a, row0);
+        group = group_of_warp(a, row0);
     } else {
         group = 0;
         n_tok = 0;
@@ -84,7 +84,7 @@ shared_any_kernel(const Args a, const int aligned) {
             ml[0] = -INFINITY;
             ml[1] = 0.f;
         }
-    const Span span = shared_span(a, group, span_scratch);
+    const Span span = shared_span(a, group);
 
     // this thread's row: eight threads each
     const int r = tid >> 3, sub = tid & 7;

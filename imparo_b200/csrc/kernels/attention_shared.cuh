@@ -39,15 +39,15 @@ __device__ __forceinline__ int group_of(const Args& a, int t) {
     const int g = lo - 1;
     return g >= 0 && t < a.group_start[g + 1] ? g : -1;
 }
-// The group of one row for a whole CTA: with few groups every thread looks at one, which is one trip to memory instead of a search's.
-__device__ __forceinline__ int group_of_cta(const Args& a, int t, int* scratch) {
-    if (a.n_groups > (int)blockDim.x) return group_of(a, t);
-    if (threadIdx.x == 0) *scratch = -1;
-    __syncthreads();
-    const int g = threadIdx.x;
-    if (g < a.n_groups && a.group_start[g] <= t && t < a.group_start[g + 1]) *scratch = g;
-    __syncthreads();
-    return *scratch;
+// The same by a warp that is together: few groups are looked at all at once, one trip to memory instead of a search's.
+__device__ __forceinline__ int group_of_warp(const Args& a, int t) {
+    if (a.n_groups > 128) return group_of(a, t);
+    for (int base = 0; base < a.n_groups; base += 32) {
+        const int g = base + (threadIdx.x & 31);
+        const unsigned found = __ballot_sync(0xffffffffu, g < a.n_groups && a.group_start[min(g, a.n_groups - 1)] <= t && t < a.group_start[min(g, a.n_groups - 1) + 1]);
+        if (found) return base + __ffs(found) - 1;
+    }
+    return -1;
 }
 __device__ __forceinline__ const int* table_row(const Args& a, int t, int kernel) {
     const int item = a.item_of_token[t];
@@ -61,26 +61,22 @@ __device__ __forceinline__ int first_seen(const Args& a, int pos) { return a.win
 
 // The keys [first, end) that the shared stretches take for a group: those of its shared positions that every row of it sees (rows
 // without a position, pos < 0, aside).  Each row takes the rest of what it sees, on both sides of them, with its own ones, so the
-// shared stretches need no mask by row and whatever a row does not see never meets its weights.  All threads call it; the result is
-// the same for every launch of the same arrays.
+// shared stretches need no mask by row and whatever a row does not see never meets its weights.  Every warp finds it by itself (no
+// barrier); the result is the same for every launch of the same arrays.
 struct Span { int first, end; };
-__device__ __forceinline__ Span shared_span(const Args& a, int g, int* scratch /* 2 */) {
-    if (g < 0) return Span{0, 0};                                  // (the same for the whole CTA)
-    if (threadIdx.x == 0) { scratch[0] = 0; scratch[1] = max(0, a.shared[g]); }
-    __syncthreads();
+__device__ __forceinline__ Span shared_span(const Args& a, int g) {
+    if (g < 0) return Span{0, 0};
     int start, end;
     group_rows(a, g, start, end);
-    int lo = 0, hi = 0x7fffffff;
-    for (int t = start + threadIdx.x; t < end; t += blockDim.x) {
+    int lo = 0, hi = max(0, a.shared[g]);
+#pragma unroll 4
+    for (int t = start + (threadIdx.x & 31); t < end; t += 32) {
         const int pos = a.positions[t];
         if (pos >= 0) { lo = max(lo, first_seen(a, pos)); hi = min(hi, pos + 1); }
     }
     lo = __reduce_max_sync(0xffffffffu, lo);
     hi = __reduce_min_sync(0xffffffffu, hi);
-    if ((threadIdx.x & 31) == 0) { atomicMax(&scratch[0], lo); atomicMin(&scratch[1], hi); }
-    __syncthreads();
-    const Span s{scratch[0], scratch[1]};
-    return s.first < s.end ? s : Span{0, 0};
+    return lo < hi ? Span{lo, hi} : Span{0, 0};
 }
 // A row's own keys, counted through: the first `before` of them lie before the shared ones.
 struct Own {

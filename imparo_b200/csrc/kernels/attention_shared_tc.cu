@@ -122,7 +122,6 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     using C = Shape<HD>;
     constexpr int NB = C::NB, ST = C::STAGES, NT = C::TILES, SB = C::S_BUFS;
     extern __shared__ __align__(1024) uint8_t tc_smem_raw[];
-    __shared__ int span_scratch[2];
     uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)tc_smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* q_s = smem;                                     // [NT][Q_BYTES]
     uint8_t* k_s = q_s + NT * C::Q_BYTES;                    // [ST][KEY_BYTES]
@@ -159,7 +158,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     const int log_r = row_tiles > 2 ? 2 : row_tiles - 1, R = 1 << log_r;   // tile x: rows x % R, every phases-th step from x / R on
     const int phases = NT >> log_r;
     const int n_tiles = R > 2 ? row_tiles : NT;              // (a fourth tile without rows does nothing)
-    const Span span = shared_span(a, group, span_scratch);
+    const Span span = shared_span(a, group);
     const int per_chunk = a.chunk_shared / STEP;
     const int first_step = span.first / STEP + chunk * per_chunk;
     const int all_steps = (span.end + STEP - 1) / STEP;
@@ -565,7 +564,6 @@ template <int HD, bool JOIN, bool WIDE>
 __global__ void __launch_bounds__(OWN_WARPS * 32, HD == 64 ? 4 : (WIDE ? 2 : 3))
 own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __restrict__ sinks, const int n_splits) {
     constexpr int NB = HD / 64, KB = HD / 32;                // 64-dim blocks (values), 32-dim blocks (keys)
-    __shared__ int span_scratch[3];
     constexpr int HEADS = WIDE ? 16 : 8, SLABS = HD == 64 && !WIDE ? 2 : 1;      // 16 keys each, all loads of a turn at once
     __shared__ float w_m[OWN_WARPS][HEADS], w_l[OWN_WARPS][HEADS];
     __shared__ __align__(16) float w_o[OWN_WARPS][HEADS][HD + 4];
@@ -576,8 +574,8 @@ own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __rest
     const int kvh = blockIdx.x / head_tiles, head0 = kvh * G + blockIdx.x % head_tiles * 16, n_heads = min(16, kvh * G + G - head0);
     const int t = blockIdx.y, split = blockIdx.z;
     const int pos = a.positions[t], item = a.item_of_token[t];           // (on their way while the group is found)
-    const int group = group_of_cta(a, t, span_scratch + 2);
-    const Span span = shared_span(a, group, span_scratch);
+    const int group = group_of_warp(a, t);
+    const Span span = shared_span(a, group);
     const Own own = own_keys(a, pos, span);
     const int k0 = (int)min((long long)split * a.chunk_own, (long long)own.count);
     const int k1 = split + 1 == a.n_own ? own.count : (int)min((long long)k0 + a.chunk_own, (long long)own.count);
