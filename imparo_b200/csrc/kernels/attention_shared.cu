@@ -275,6 +275,8 @@ extern "C" int imparo_attention_shared(const void* q, long long q_stride, const 
     a.n_rows = n_rows; a.n_items = n_items; a.n_groups = n_groups; a.max_blocks = max_blocks; a.page_size = page_size;
     a.n_pages = n_pages; a.window = window; a.nh = nh; a.nkv = nkv; a.hd = hd;
     a.chunk_shared = chunk_shared; a.n_shared = n_shared; a.chunk_own = chunk_own; a.n_own = n_own; a.scale = scale;
+    const long long positions_of_table = (long long)max_blocks * page_size;
+    a.most_pos = (int)(positions_of_table < 0x7ffffffell ? positions_of_table : 0x7ffffffell);
     int rc = dtype == IMPARO_DT_BF16 ? sp::launch_tc(a, out, sink_values, stream) : -8;
     if (rc == 0 && n_own == 1) return 0;                     // its second kernel has joined everything
     if (rc == -8) rc = dtype == IMPARO_DT_F32 ? sp::launch_any<float>(a, stream) : sp::launch_any<__nv_bfloat16>(a, stream);

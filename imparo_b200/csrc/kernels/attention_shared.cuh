@@ -21,6 +21,7 @@ struct Args {
     long long q_stride;            // elements between rows of q
     int n_rows, n_items, n_groups, max_blocks, page_size, n_pages, window, nh, nkv, hd;
     int chunk_shared, n_shared, chunk_own, n_own;
+    int most_pos;                  // the first position that the table has no block for: later ones are taken for it
     float scale;
 };
 
@@ -71,20 +72,22 @@ __device__ __forceinline__ Span shared_span(const Args& a, int g) {
     int lo = 0, hi = max(0, a.shared[g]);
 #pragma unroll 4
     for (int t = start + (threadIdx.x & 31); t < end; t += 32) {
-        const int pos = a.positions[t];
+        const int pos = min(a.positions[t], a.most_pos);
         if (pos >= 0) { lo = max(lo, first_seen(a, pos)); hi = min(hi, pos + 1); }
     }
     lo = __reduce_max_sync(0xffffffffu, lo);
     hi = __reduce_min_sync(0xffffffffu, hi);
     return lo < hi ? Span{lo, hi} : Span{0, 0};
 }
-// A row's own keys, counted through: the first `before` of them lie before the shared ones.
+// A row's own keys, counted through: the first `before` of them lie before the shared ones.  (A position far beyond the table is an
+// error that the first key without a block reports; without the bound the row would look up every one of up to 2^31 keys.)
 struct Own {
     int lo, before, skip, count;
     __device__ __forceinline__ int key(int i) const { return lo + i + (i < before ? 0 : skip); }
 };
 __device__ __forceinline__ Own own_keys(const Args& a, int pos, Span s) {
     Own o;
+    pos = min(pos, a.most_pos);
     o.lo = first_seen(a, pos);
     o.before = s.first < s.end ? s.first - o.lo : 0x7fffffff;      // (a row sees all of the span: lo <= first, end <= pos + 1)
     o.skip = s.end - s.first;

@@ -233,6 +233,19 @@ class TestRows:
             with pytest.raises(ops.KernelError):
                 ops.read_status(b.status)
 
+    def test_positions_far_beyond_the_table_are_reported(self, dtype, hd):
+        """At once, not after two thousand million keys; the other rows are as they were."""
+        for which, window in ((slice(1, 2), None), (slice(0, 4), None), (slice(2, 3), 100)):
+            b = Batch([(4, 200), (2, 50)], 30, 4, 2, hd, dtype)
+            want = b.run(window=window)
+            b.positions[which] = 0x7fffffff
+            if which.stop == 4:
+                b.shared[0] = 0x7fffffff
+            got = b.run(window=window, check=False)
+            with pytest.raises(ops.KernelError):
+                ops.read_status(b.status)
+            assert torch.equal(got[4:], want[4:])
+
     def test_captured_and_replayed(self, dtype, hd):
         b = Batch([(4, 300), (2, 64)], lambda r: 9 + r, 4, 2, hd, dtype)
         plan = ops.shared_prefix_plan(6, 2, 4, 2, hd, dtype, 300, 20)
