@@ -54,7 +54,7 @@ __device__ __forceinline__ Item read_item(const Args& a, int r) {
         const int p = a.parent[r];
         if (p >= 0 && p < a.n_items) {
             it.from = p;
-            it.shared_blocks = max(0, a.shared[r]) / a.page_size;
+            it.shared_blocks = min(max(0, a.shared[r]), it.length) / a.page_size;           // (new positions never go to a parent's page)
         }
     }
     return it;
@@ -94,6 +94,11 @@ step_tables_kernel(const Args a) {
 #pragma unroll
     for (int i = 0; i < THREADS / 32; ++i) { tokens += part[0][i]; pages += part[1][i]; }
 
+    // a page that is held: none where the arena has no such page
+    auto listed = [&](int page, int r) -> int {
+        if (page >= a.n_pages) report(a.status, IMPARO_ST_PAGE_RANGE, 64, r, page);
+        return page < 0 || page >= a.n_pages ? -1 : page;
+    };
     for (int r = r0; r < r1; ++r) {
         const Item it = read_item(a, r);
         int* row = a.table + (size_t)r * a.width;
@@ -103,10 +108,11 @@ step_tables_kernel(const Args a) {
             if (it.count > 0 && it.last < (it.length + it.count + a.page_size - 1) / a.page_size)
                 report(a.status, IMPARO_ST_STEP_SIZE, 61, r, it.length + it.count);
             if (a.parent && a.parent[r] >= a.n_items) report(a.status, IMPARO_ST_STEP_SIZE, 62, r, a.parent[r]);
+            if (it.from != r && a.shared[r] / a.page_size > it.shared_blocks) report(a.status, IMPARO_ST_STEP_SIZE, 66, r, a.shared[r]);
         }
         // blocks without new positions: as held
         for (int b = tid; b < a.width; b += THREADS)
-            if (b < it.first || b >= it.last) row[b] = max(-1, held_page(a, it, r, b));
+            if (b < it.first || b >= it.last) row[b] = listed(held_page(a, it, r, b), r);
         // blocks with new positions: the missing pages from the free list, in order; every warp counts, one writes
         long long next = pages;
         for (int b0 = it.first; b0 < it.last; b0 += 32) {
@@ -119,9 +125,9 @@ step_tables_kernel(const Args a) {
                 page = at < a.n_free ? a.free_pages[at] : -1;
                 if (warp == 0 && (page < 0 || page >= a.n_pages))
                     report(a.status, at < a.n_free ? IMPARO_ST_PAGE_RANGE : IMPARO_ST_STEP_SIZE, 63, r, page);
-                if (page >= a.n_pages) page = -1;
+                if (page < 0 || page >= a.n_pages) page = -1;
             }
-            if (warp == 0 && b < it.last) row[b] = page;
+            if (warp == 0 && b < it.last) row[b] = listed(page, r);
             next += __popc(mask);
         }
         __syncthreads();                                       // the row is written: the tokens read it
@@ -130,11 +136,9 @@ step_tables_kernel(const Args a) {
             if (t >= a.n_tokens) break;
             const int pos = it.length + i, b = pos / a.page_size;
             const int page = b < a.width ? row[b] : -1;
-            const bool good = page >= 0 && page < a.n_pages;
             a.positions[t] = pos;
             a.item_of_token[t] = r;
-            a.slots[t] = good ? (long long)page * a.page_size + pos % a.page_size : -1;
-            if (page >= a.n_pages) report(a.status, IMPARO_ST_PAGE_RANGE, 64, r, page);
+            a.slots[t] = page >= 0 ? (long long)page * a.page_size + pos % a.page_size : -1;
         }
         tokens += it.count;
         pages = next;

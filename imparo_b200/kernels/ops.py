@@ -1625,8 +1625,8 @@ def step_tables(lengths, counts, free_pages, held, page_size, n_pages, table, po
     page_size + place) per token; entries behind the last token get position -1 (which attends to nothing), item 0 and slot -1.
     taken (int32 [1]): how many of the free pages are now in use.
 
-    A free list that is too short, a table or token arrays that are too narrow, negative lengths and pages outside [0, n_pages) are
-    recorded in the status word (read_status raises); nothing is written out of range, what has no page gets -1.  What is written must
+    A free list that is too short, a table or token arrays that are too narrow, negative lengths, whole shared pages beyond lengths[r]
+    and pages outside [0, n_pages) are recorded in the status word (read_status raises); nothing is written out of range, what has no page gets -1.  What is written must
     not overlap what is read."""
     _placed("step_tables", lengths, counts, free_pages, held, table, positions, item_of_token, row_start, slots, taken, status, parent, shared)
     _need(held.dim() == 2 and table.dim() == 2, "step_tables: held and table must be [items, blocks]")

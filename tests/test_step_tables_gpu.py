@@ -199,3 +199,22 @@ def test_refusals():
                    dict(table=i32(3, 8)[:, :5])):
         with pytest.raises(ops.KernelError):
             ops.step_tables(**{**good, **change})
+
+
+def test_pages_that_do_not_exist_are_left_out_of_the_table():
+    """Held ones of past positions too, and negative ones of the free list; the rest of the step is as ever."""
+    outs, status = device_call(np.array([40, 5]), np.array([10, 3]), np.array([-5, 6, 7]), np.array([[3, 99, -1, -1], [2, -1, -1, 77]]), 16, 10, 4, 13)
+    with pytest.raises(ops.KernelError):
+        ops.read_status(status)
+    assert outs[0].tolist() == [[3, -1, -1, 6], [2, -1, -1, -1]] and outs[5].tolist() == [2]
+    assert outs[4].tolist() == [-1] * 8 + [96, 97] + [37, 38, 39]
+    assert outs[1].tolist() == list(range(40, 50)) + [5, 6, 7]
+
+
+def test_new_positions_never_go_to_a_parents_page():
+    """More shared positions than the item holds: reported, and its new ones take a page of their own."""
+    outs, status = device_call(np.array([40, 20]), np.array([1, 2]), np.array([8, 9]), np.array([[3, 4, 5], [-1, -1, -1]]), 16, 10, 3, 3,
+                               parent=[-1, 0], shared=[0, 40])
+    with pytest.raises(ops.KernelError):
+        ops.read_status(status)
+    assert outs[0].tolist() == [[3, 4, 5], [3, 8, -1]] and outs[4].tolist() == [5 * 16 + 8, 8 * 16 + 4, 8 * 16 + 5]
