@@ -368,7 +368,7 @@ sample_filtered_kernel(const Args a) {
     }
     const float topf = unordered((uint32_t)(top >> 32));
     Weights weight;
-    weight.top = topf; weight.topf = topf; weight.rate = STEPS * 1.4426950408889634074 / (double)temp; weight.least = topf - 43.5f * temp; weight.table = s.table;
+    weight.top = topf; weight.topf = topf; weight.rate = STEPS * 1.4426950408889634074 / (double)temp; weight.least = topf < INFINITY ? topf - 43.5f * temp : INFINITY; weight.table = s.table;
     weight.shift = a.shift;
     // Entries below floor_v lie beyond every cut: the last bin is theirs.
     float floor_v = from > ALL ? unordered((uint32_t)(from >> 32)) : -INFINITY;
@@ -497,7 +497,8 @@ sample_filtered_kernel(const Args a) {
         if (!a.min_p || !(a.min_p[r] > 0.f)) return ALL;
         const float p = a.min_p[r];
         if (p > 1.f) return top;                                   // only the first largest entry stays
-        const float bound = __double2float_ru((double)topf + (double)temp * log((double)p));
+        // (what is below an infinite logit weighs nothing, at an infinite temperature too)
+        const float bound = topf < INFINITY ? __double2float_ru((double)topf + (double)temp * log((double)p)) : topf;
         return bound > -INFINITY ? (u64)ordered(bound + 0.0f) << 32 : ALL;
     };
 

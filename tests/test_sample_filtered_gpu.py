@@ -145,6 +145,22 @@ def test_nan_infinities_and_masks():
     assert got[3] == (0, 0) and got[4] == (0, 0) and got[5] == (4000, 1)
 
 
+@pytest.mark.parametrize("vocab", [900, 70001])
+def test_infinite_logits_take_all_the_weight_at_any_temperature(vocab):
+    rng = np.random.default_rng(7)
+    t, u, k, p, m = settings(rng, 28, vocab)
+    x = rng.standard_normal((28, vocab)).astype(np.float32)
+    x[:, [5, 300, vocab - 1]] = np.inf
+    x = torch.tensor(x, device=DEV)
+    want = check(x, t, u, k, p, m)
+    i32, f32 = (lambda v: torch.tensor(np.asarray(v), dtype=torch.int32, device=DEV)), (lambda v: torch.tensor(np.asarray(v), dtype=torch.float32, device=DEV))
+    for hot in (1e30, np.inf):
+        out, kept = i32(np.zeros(28)), i32(np.zeros(28))
+        ops.sample_filtered(x, f32(np.where(t > 0, hot, 0)), f32(u), out, top_k=i32(k), top_p=f32(p), min_p=f32(m), kept=kept)
+        # (top-k may leave other entries of weight 0, where there are more than three: the same ones at any temperature)
+        assert list(zip(out.tolist(), kept.tolist())) == want
+
+
 def test_single_settings_at_their_limits():
     rng = np.random.default_rng(8)
     vocab = 3001
