@@ -144,6 +144,18 @@ def test_rows_of_a_group(dtype, hd, rows):
     Batch([(rows, 333)], lambda r: 1 + r % 5, 4, 1, hd, dtype, seed=rows).check()
 
 
+@pytest.mark.parametrize("dtype,hd", [(torch.float32, 32), (torch.bfloat16, 64), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("group", [33, 64, 100, 128, 130])
+def test_many_heads_to_a_kv_head(dtype, hd, group):
+    Batch([(3, 190), (2, 64)], lambda r: 1 + 40 * r, 2 * group, 2, hd, dtype, extra=1, seed=group).check()
+
+
+@pytest.mark.parametrize("page", [48, 96, 192])
+@pytest.mark.parametrize("window", [None, 150])
+def test_page_sizes_that_are_no_power_of_two(page, window):
+    Batch([(4, 500), (2, 199)], lambda r: 3 + 70 * r, 4, 2, 64, torch.bfloat16, page=page).check(window=window)
+
+
 @pytest.mark.parametrize("page", [1, 5, 16, 32, 64, 128, 256])
 @pytest.mark.parametrize("dtype,hd", [(torch.float32, 64), (torch.bfloat16, 64), (torch.bfloat16, 128)])
 def test_page_sizes(dtype, hd, page):
