@@ -826,6 +826,225 @@ own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __rest
     if (!JOIN && tid == 0) pdl_wait_at_end();                // this kernel completes after the one it ran beside
 }
 
+// The same for up to eight query heads to a kv head, joined at once: a CTA takes a token and `per` of its kv heads, one to a warp.  A warp
+// copies its keys and values into a ring of its own, up to RING turns of 16 keys ahead, so that the memory's latency is paid once and not a
+// turn; no result leaves it: the partial results of the shared keys are read by the lanes that hold the same dims.  132 rows of 8 kv heads of
+// 128 over 8,000 shared positions and up to 200 own ones 59 us with the kernel before, of which this one about 20 (39 by a CTA per kv head).
+constexpr int OWN_DIMS = 512, TURN = 16, LOOKED = 1024;      // dims of a CTA's heads; LOOKED keys' places are looked up at once
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+constexpr size_t own_ring_bytes(int turns, int dims) { return (size_t)turns * TURN * dims * 4; }
+
+template <int HD, int RING>
+__global__ void __launch_bounds__(OWN_DIMS / HD * 32, 2)
+own_ring_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __restrict__ sinks, const int n_splits) {
+    constexpr int NB = HD / 64, KB = HD / 32;
+    constexpr uint32_t ROW = HD * 2, SLAB = TURN * ROW;
+    extern __shared__ __align__(128) uint8_t ring[];         // [warp][RING][keys, values][TURN][ROW]
+    __shared__ int where[LOOKED];
+    pdl_trigger();
+    pdl_no_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tg = lane & 3;
+    const int G = a.nh / a.nkv, t = blockIdx.y, kvh = blockIdx.x * (blockDim.x >> 5) + warp;
+    const int pos = a.positions[t], item = a.item_of_token[t];
+    const int group = group_of_warp(a, t);
+    const Span span = shared_span(a, group);
+    const Own own = own_keys(a, pos, span);
+    const bool there_is_a_row = item >= 0 && item < a.n_items;
+    if (own.count > 0 && !there_is_a_row && threadIdx.x == 0) report(a.status, IMPARO_ST_PAGE_RANGE, 84, t, item);
+    const int count = there_is_a_row ? own.count : 0;
+    const int* tab = a.table + (size_t)(there_is_a_row ? item : 0) * a.max_blocks;
+    const size_t kvw = (size_t)a.nkv * HD;
+    const uint8_t* mine = ring + warp * (RING * 2 * SLAB);
+    // copies: lane >> 3 is the key (and every fourth from it), lane & 7 the 16 bytes of each 128; their places in shared memory are such that
+    // neither the copies nor the fragments' reads meet a bank twice
+    const __nv_bfloat16* kc = reinterpret_cast<const __nv_bfloat16*>(a.k) + (size_t)kvh * HD + (lane & 7) * 8;
+    const __nv_bfloat16* vc = reinterpret_cast<const __nv_bfloat16*>(a.v) + (size_t)kvh * HD + (lane & 7) * 8;
+    auto fetch = [&](int turn) {                             // a turn of the LOOKED keys
+        const uint32_t to = smem_u32(mine) + turn % RING * (2 * SLAB);
+#pragma unroll
+        for (int c = 0; c < TURN / 4; ++c) {
+            const int key = (lane >> 3) + 4 * c, row = where[turn * TURN + key];
+            if (row >= 0) {
+#pragma unroll
+                for (int d = 0; d < NB; ++d) {
+                    copy16(to + key * ROW + d * 128 + (((lane & 7) ^ ((key & 1) << 2)) << 4), kc + (size_t)row * kvw + d * 64);
+                    copy16(to + SLAB + key * ROW + d * 128 + (((lane & 7) ^ (key & 6)) << 4), vc + (size_t)row * kvw + d * 64);
+                }
+            }
+        }
+    };
+    const int head0 = kvh * G;
+    uint4 qa[KB];                                            // the queries: head g, dims 32 b + 8 tg .. + 7
+    {
+        const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)t * a.q_stride + (size_t)head0 * HD + tg * 8;
+#pragma unroll
+        for (int b = 0; b < KB; ++b) qa[b] = g < G ? *reinterpret_cast<const uint4*>(q + (size_t)g * HD + b * 32) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    float o[NB * 8][2];                                      // head g, dims 64 nb + 8 (2 tg + e) + i at [nb * 8 + i][e]
+#pragma unroll
+    for (int i = 0; i < NB * 8; ++i) o[i][0] = o[i][1] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    const float sl2 = a.scale * LOG2E;
+    for (int done = 0; done < count; done += LOOKED) {
+    const int known = min(LOOKED, count - done), turns = (known + TURN - 1) / TURN;
+    if (done > 0) __syncthreads();                           // (every warp is through with the places before)
+    for (int i = threadIdx.x; i < turns * TURN; i += blockDim.x) {
+        int row = -1;
+        if (i < known) {
+            const int key = own.key(done + i), block = key / a.page_size;
+            const int page = block < a.max_blocks ? tab[block] : -1;
+            if (page >= 0 && page < a.n_pages) row = page * a.page_size + key % a.page_size;
+            else report(a.status, IMPARO_ST_PAGE_RANGE, 85, t, page);
+        }
+        where[i] = row;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < RING - 1; ++i) {
+        if (i < turns) fetch(i);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    for (int turn = 0; turn < turns; ++turn) {
+        __syncwarp();                                        // (the turn whose place the next one takes has been read by all lanes)
+        if (turn + RING - 1 < turns) fetch(turn + RING - 1);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
+        const unsigned there = __ballot_sync(0xffffffffu, where[turn * TURN + (lane & 15)] >= 0) & 0xffffu;
+        __syncwarp();                                        // every lane's copies of this turn have arrived
+        const uint8_t* ks = mine + turn % RING * (2 * SLAB);
+        const uint8_t* vs = ks + SLAB;
+        float s[2][2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int d = 0; d < KB; ++d) {
+                const uint4 kf = *reinterpret_cast<const uint4*>(ks + (n * 8 + g) * ROW + (d >> 1) * 128 + ((((d & 1) << 2 | tg) ^ ((g & 1) << 2)) << 4));
+                mma16816(c, qa[d].x, 0u, qa[d].y, 0u, kf.x, kf.y);
+                mma16816(c, qa[d].z, 0u, qa[d].w, 0u, kf.z, kf.w);
+            }
+            s[n][0] = c[0];
+            s[n][1] = c[1];
+        }
+        uint4 vf[4][NB];                                     // keys 2 tg, 2 tg + 1, 2 tg + 8, 2 tg + 9
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int key = 2 * tg + (u & 1) + (u >> 1) * 8;
+#pragma unroll
+            for (int d = 0; d < NB; ++d) {
+                vf[u][d] = *reinterpret_cast<const uint4*>(vs + key * ROW + d * 128 + ((g ^ (key & 6)) << 4));
+                if (there != 0xffffu && !((there >> key) & 1u)) vf[u][d] = make_uint4(0u, 0u, 0u, 0u);       // (nothing was copied)
+            }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                s[n][e] = (there >> (n * 8 + 2 * tg + e)) & 1u ? s[n][e] * sl2 : -INFINITY;
+                mx = fmaxf(mx, s[n][e]);
+            }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float m_new = fmaxf(m, mx), corr = m == -INFINITY ? 0.f : ex2(m - m_new), base = m_new == -INFINITY ? 0.f : m_new;
+        m = m_new;
+        l *= corr;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) { s[n][e] = ex2(s[n][e] - base); l += s[n][e]; }
+#pragma unroll
+        for (int i = 0; i < NB * 8; ++i) { o[i][0] *= corr; o[i][1] *= corr; }
+        const uint32_t p0 = pack_bf16(s[0][0], s[0][1]), p2 = pack_bf16(s[1][0], s[1][1]);
+#pragma unroll
+        for (int d = 0; d < NB; ++d) {
+            const uint32_t x0[4] = {vf[0][d].x, vf[0][d].y, vf[0][d].z, vf[0][d].w}, x1[4] = {vf[1][d].x, vf[1][d].y, vf[1][d].z, vf[1][d].w};
+            const uint32_t x2[4] = {vf[2][d].x, vf[2][d].y, vf[2][d].z, vf[2][d].w}, x3[4] = {vf[3][d].x, vf[3][d].y, vf[3][d].z, vf[3][d].w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t pick = i & 1 ? 0x7632u : 0x5410u;
+                float c[4] = {o[d * 8 + i][0], o[d * 8 + i][1], 0.f, 0.f};
+                mma16816(c, p0, 0u, p2, 0u, __byte_perm(x0[i >> 1], x1[i >> 1], pick), __byte_perm(x2[i >> 1], x3[i >> 1], pick));
+                o[d * 8 + i][0] = c[0];
+                o[d * 8 + i][1] = c[1];
+            }
+        }
+    }
+    }
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    // the shared stretches that hold anything for this row's group
+    int live = 0;
+    if (span.first < span.end) {
+        const int per_chunk = a.chunk_shared / STEP, steps = (span.end + STEP - 1) / STEP - span.first / STEP;
+        live = min(a.n_shared, (steps + per_chunk - 1) / per_chunk);
+    }
+    pdl_wait();                                              // the kernel that makes the partial results is complete
+    if (g >= G) return;
+    const size_t row = (size_t)t * a.nh + head0 + g;
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row * n_splits;
+    const float* part = a.part_acc + row * n_splits * HD + tg * 16;
+    constexpr int AHEAD = 2;                                 // partial results on their way at once
+    for (int s0 = 0; s0 < live; s0 += AHEAD) {
+        float2 v[AHEAD];
+        float4 x[AHEAD][NB][4];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            v[u] = s0 + u < live ? __ldcg(ml + s0 + u) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int d = 0; d < NB; ++d)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    x[u][d][c] = s0 + u < live ? __ldcg(reinterpret_cast<const float4*>(part + (size_t)(s0 + u) * HD + d * 64) + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float m_new = m;
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) m_new = fmaxf(m_new, v[u].y != 0.f ? v[u].x * LOG2E : -INFINITY);
+        const float corr = m == -INFINITY ? 0.f : ex2(m - m_new);
+        m = m_new;
+        l *= corr;
+#pragma unroll
+        for (int i = 0; i < NB * 8; ++i) { o[i][0] *= corr; o[i][1] *= corr; }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            if (v[u].y == 0.f) continue;                     // (a result of sum 0 has no values)
+            const float f = ex2(v[u].x * LOG2E - m);
+            l += v[u].y * f;
+#pragma unroll
+            for (int d = 0; d < NB; ++d)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {                // dims 64 d + 16 tg + 4 c ..: e = c / 2, i from 4 (c % 2) on
+                    o[d * 8 + 4 * (c & 1)][c >> 1] += x[u][d][c].x * f;
+                    o[d * 8 + 4 * (c & 1) + 1][c >> 1] += x[u][d][c].y * f;
+                    o[d * 8 + 4 * (c & 1) + 2][c >> 1] += x[u][d][c].z * f;
+                    o[d * 8 + 4 * (c & 1) + 3][c >> 1] += x[u][d][c].w * f;
+                }
+        }
+    }
+    if (sinks) {
+        const float sink = sinks[head0 + g] * LOG2E, m_new = fmaxf(m, sink), corr = m == -INFINITY ? 0.f : ex2(m - m_new);
+        l = l * corr + ex2(sink - m_new);
+#pragma unroll
+        for (int i = 0; i < NB * 8; ++i) { o[i][0] *= corr; o[i][1] *= corr; }
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+    for (int d = 0; d < NB; ++d)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            uint4 w;
+            w.x = pack_bf16(o[d * 8][e] * inv, o[d * 8 + 1][e] * inv);
+            w.y = pack_bf16(o[d * 8 + 2][e] * inv, o[d * 8 + 3][e] * inv);
+            w.z = pack_bf16(o[d * 8 + 4][e] * inv, o[d * 8 + 5][e] * inv);
+            w.w = pack_bf16(o[d * 8 + 6][e] * inv, o[d * 8 + 7][e] * inv);
+            *reinterpret_cast<uint4*>(out + row * HD + d * 64 + 8 * (2 * tg + e)) = w;
+        }
+}
+
 // A [rows, cols] bfloat16 matrix without gaps, tiles of box_rows x 64 elements, 128-byte swizzle.
 static int encode(const void* ptr, uint64_t rows, uint64_t cols, uint32_t box_rows, CUtensorMap* out) {
     static PFN_cuTensorMapEncodeTiled fn = nullptr;          // (found once; two threads that look at the same time find the same)
@@ -852,20 +1071,42 @@ static int launch_hd(const Args& a, __nv_bfloat16* out, const float* sinks, cuda
     if (rc) return rc;
     rc = encode(a.v, rows, cols, (uint32_t)box, &mv);
     if (rc) return rc;
-    static bool configured[64] = {};                         // the attribute is the device's
+    constexpr int DEEP = 4, SHALLOW = 3;                     // turns of a ring: a CTA per SM, two CTAs per SM
+    static int sms[65] = {};                                 // by device; the attributes below are the device's too
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return (int)e;
-    if (device < 0 || device >= 64 || !configured[device]) {
+    const int slot = device >= 0 && device < 64 ? device : 64;
+    if (slot == 64 || sms[slot] == 0) {
         e = cudaFuncSetAttribute(shared_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<HD>::SMEM);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(own_ring_kernel<HD, DEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)own_ring_bytes(DEEP, OWN_DIMS));
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(own_ring_kernel<HD, SHALLOW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)own_ring_bytes(SHALLOW, OWN_DIMS));
+        int n = 0;
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device);
         if (e != cudaSuccess) return (int)e;
-        if (device >= 0 && device < 64) configured[device] = true;
+        sms[slot] = n;
     }
     const int n_splits = a.n_own == 1 ? a.n_shared : a.n_shared + a.n_own;
     const int tokens = Shape<HD>::TILES * TQ;
     const long long units = (a.n_rows + tokens - 1) / tokens + a.n_groups - 1;       // every group may end a tile early
     e = launch(shared_tc_kernel<HD>, dim3(a.nkv, a.n_shared, (unsigned)units), dim3(Shape<HD>::THREADS), Shape<HD>::SMEM, stream, mk, mv, a, n_splits);
     if (e != cudaSuccess) return (int)e;
+    int per = OWN_DIMS / HD;                                 // kv heads of a CTA that takes a row's own keys by rings
+    while (a.nkv % per != 0) --per;
+    const long long ctas = (long long)a.nkv / per * a.n_rows;
+    // Rings, as soon as a CTA per token and 512 dims gives half of the SMs something to do: 256 rows of 8 kv heads of 64 over 20,000 shared
+    // positions and up to 200 own ones 92 us (109 by a CTA per kv head), 128 rows 56 (64), 80 rows 48 (47); below, one warp's turns
+    // take longer than four warps' (64 rows over 32,768: 51 against 48, 40 rows over 8,000: 30 against 25).  Up to a CTA per SM the
+    // shared memory is such that no two come to the same SM (128 rows: 56; with two to an SM, where they would go first, 65).
+    if (G <= 8 && a.n_own == 1 && 2 * ctas > sms[slot]) {
+        const bool few = ctas <= sms[slot];
+        const size_t smem = own_ring_bytes(few ? DEEP : SHALLOW, few ? OWN_DIMS : per * HD);
+        e = launch(few ? own_ring_kernel<HD, DEEP> : own_ring_kernel<HD, SHALLOW>, dim3(a.nkv / per, a.n_rows), dim3(32 * per), smem, stream, a,
+                   out, sinks, n_splits);
+        return e == cudaSuccess ? 0 : (int)e;
+    }
     const dim3 grid(a.nkv * head_tiles, a.n_rows, a.n_own);
     auto own = G > 8 ? (a.n_own == 1 ? own_tc_kernel<HD, true, true> : own_tc_kernel<HD, false, true>)
                      : (a.n_own == 1 ? own_tc_kernel<HD, true, false> : own_tc_kernel<HD, false, false>);

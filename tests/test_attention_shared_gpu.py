@@ -286,6 +286,62 @@ def test_many_rows_and_long_prefix():
     b.check()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows", [90, 170])
+class TestManyRows:
+    """So many rows that a row's own keys are taken by one CTA for several kv heads, one or two to an SM."""
+
+    @pytest.mark.parametrize("nh,nkv", [(2, 2), (6, 2), (16, 2), (6, 3), (33, 11)])
+    def test_heads(self, hd, rows, nh, nkv):
+        Batch([(rows, 100)], lambda r: 1 + 29 * r % 71, nh, nkv, hd, torch.bfloat16).check()
+
+    @pytest.mark.parametrize("window", [None, 1, 150])
+    def test_groups_of_all_kinds(self, hd, rows, window):
+        b = Batch([(rows - 8, 333), (0, 5), (3, 0), (1, 70), (2, 48)], lambda r: 1 + 37 * r % 200, 8, 2, hd, torch.bfloat16, extra=2)
+        b.positions[3] = b.positions[rows - 1] = -1
+        b.positions[7] = b.positions[7] // 2 if window is None else b.positions[7]
+        got = b.check(window=window)
+        assert not got[3].any() and not got[rows - 1].any()
+        b.check(window=window, sinks=torch.tensor([-50.0, -2.0, 0.0, 1.0, 3.0, 8.0, 30.0, 80.0], device=DEV))
+
+    @pytest.mark.parametrize("page", [1, 5, 64])
+    def test_page_sizes(self, hd, rows, page):
+        Batch([(rows - 5, 130), (5, 64)], lambda r: 1 + r % 50, 4, 2, hd, torch.bfloat16, page=page).check()
+
+    def test_long_rows_among_short_ones(self, hd, rows):
+        """More own keys than are looked up at once, just as many, one more."""
+        b = Batch([(rows, 40)], lambda r: {0: 1024, 5: 1025, 9: 1023, 40: 2100, 80: 1040}.get(r, 1 + r % 20), 4, 2, hd, torch.bfloat16)
+        plan = ops.shared_prefix_plan(rows, 1, 4, 2, hd, torch.bfloat16, 40, 100)
+        assert plan.n_own == 1
+        b.check(plan=plan)
+
+    def test_a_row_does_not_feel_its_neighbours_or_what_it_may_not_see(self, hd, rows):
+        b = Batch([(rows, 100)], 37, 8, 2, hd, torch.bfloat16)
+        b.positions[2] = 119                                       # of 136
+        plan = ops.shared_prefix_plan(rows, 1, 8, 2, hd, torch.bfloat16, 100, 37)
+        want = b.run(plan=plan)
+        b.v[b.table[2, 7], 8:] = float("inf")                      # positions 120 to 127
+        b.k[b.table[2, 8]] = float("nan")
+        b.q[3:] = b.q[3:].flip(0)
+        got = b.run(plan=plan)
+        assert torch.equal(got[:3], want[:3]) and torch.equal(b.run(plan=plan), got)
+
+    @pytest.mark.parametrize("what", ["page", "unmapped", "item", "far"])
+    def test_what_is_wrong_is_reported(self, hd, rows, what):
+        b = Batch([(rows, 64)], 30, 4, 2, hd, torch.bfloat16)
+        want = b.run()
+        if what == "item":
+            b.items[2] = 9999
+        elif what == "far":
+            b.positions[2] = 0x7fffffff
+        else:
+            b.table[2, 5] = b.n_pages if what == "page" else -1
+        got = b.run(check=False)
+        with pytest.raises(ops.KernelError):
+            ops.read_status(b.status)
+        assert torch.equal(got[3:], want[3:])
+
+
 def test_no_rows():
     b = Batch([(2, 30)], 2, 4, 2, 64, torch.bfloat16)
     plan = ops.shared_prefix_plan(1, 1, 4, 2, 64, torch.bfloat16, 30, 2)
