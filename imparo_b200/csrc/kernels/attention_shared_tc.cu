@@ -5,7 +5,7 @@
 // of one kv head) as two tiles of 128 rows, and leaves each row's partial result.  The second takes each row's own keys, and joins
 // them with the partial results of the shared ones.
 //
-// On a B200, bfloat16, 32 heads in 8 groups of 64: 256 rows over 100,000 shared and up to 200 own positions 296 us (the first kernel about 260:
+// On a B200, bfloat16, 32 heads in 8 groups of 64: 256 rows over 100,000 shared and up to 200 own positions 278 us (the first kernel about 260:
 // 0.8 PFLOP/s of products, the exponential units busy for two thirds of it), 64 rows over 32,768 and up to 256 own ones 49 us.
 #include "attention_shared.cuh"
 #include "tcgen05.cuh"
