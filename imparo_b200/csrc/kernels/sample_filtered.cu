@@ -25,6 +25,7 @@
 #include "common.cuh"
 #include <cooperative_groups.h>
 #include <type_traits>
+#include <utility>
 
 namespace imparo {
 namespace sf {
@@ -218,9 +219,12 @@ sample_filtered_kernel(const Args a) {
     extern __shared__ __align__(16) uint8_t sf_smem[];
     Shared& s = *reinterpret_cast<Shared*>(sf_smem);
     float* staged = reinterpret_cast<float*>(sf_smem + ((sizeof(Shared) + 15) & ~(size_t)15));
+    cg::cluster_group cluster = cg::this_cluster();
+    // A CTA's shared memory may be touched by the others only once it runs: each says so here, and waits for all of them before its first
+    // store to another.  What lies between, the load of the stretch, hides the barrier.
+    auto started = cluster.barrier_arrive();
     pdl_trigger();
     pdl_wait();
-    cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int r = blockIdx.x / ranks;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -328,6 +332,7 @@ sample_filtered_kernel(const Args a) {
     {
         const int group = ranks > 2 ? ranks / 2 : 1;               // threads that share one
         for (int o = 1; o < group; o <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+        cluster.barrier_wait(std::move(started));
         if (tid % group == 0)
             for (int k = 0; k < ranks; ++k) *cluster.map_shared_rank(&largest[rank * (groups / ranks) + tid / group], k) = mine;
     }

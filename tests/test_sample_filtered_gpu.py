@@ -221,6 +221,30 @@ def test_captured_and_replayed_on_another_stream():
         assert list(zip(out.tolist(), kept.tolist())) == want
 
 
+@pytest.mark.parametrize("rows", [1, 3, 8, 60])
+def test_a_row_of_several_ctas_while_other_kernels_come_and_go(rows):
+    """A row's CTAs give one another what they found in their stretches as soon as all of them run, however busy the SMs are."""
+    rng = np.random.default_rng(rows)
+    vocab = 65536
+    logits = torch.tensor(rng.standard_normal((rows, vocab)) * 2, dtype=torch.float32, device=DEV)
+    settled = settings(rng, rows, vocab)
+    want = check(logits, *settled)
+    args = [torch.tensor(x, device=DEV) for x in settled]
+    calls = 40
+    outs, kepts = ([torch.full((rows,), -7, dtype=torch.int32, device=DEV) for _ in range(calls)] for _ in range(2))
+    side, a, small = torch.cuda.Stream(), torch.randn(1024, 1024, device=DEV), torch.randn(1 << 16, device=DEV)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(60):
+            a = torch.tanh(a @ a)
+            small = small * 0.5 + 1.0
+    for out, kept in zip(outs, kepts):
+        ops.sample_filtered(logits, args[0], args[1], out, top_k=args[2], top_p=args[3], min_p=args[4], kept=kept)
+    torch.cuda.synchronize()
+    for out, kept in zip(outs, kepts):
+        assert list(zip(out.tolist(), kept.tolist())) == want
+
+
 def test_no_rows():
     e = torch.empty(0, device=DEV)
     ops.sample_filtered(torch.empty(0, 100, device=DEV), e, e, torch.empty(0, dtype=torch.int32, device=DEV))
