@@ -155,7 +155,10 @@ __device__ __forceinline__ float plain_act_bf16(int kind, float z) {
 // their weight tiles (which no kernel writes).  Without the launch attribute both are no-ops.
 // Before its wait a kernel may read only what no kernel of the chain writes: weights, and the
 // batch description of the step (positions, request of a token, portion starts, state slots,
-// block tables), which the host copies to the device before the step's first kernel.  (One exception: the routed experts' down
+// block tables).  The host copies it to the device before the step's first kernel, or step_tables.cu makes it there: that operator
+// ends with a launch that waits for it in full, so that no kernel behind it starts before the description is complete.  Whoever else
+// writes such an array on the device has to do the same (launch_after): a trigger makes nothing visible to a kernel that has not waited,
+// and later kernels of the chain may be resident too.  (One exception: the routed experts' down
 // launch reads the choices of a kernel two launches back; moe.cu says what makes that safe.)
 #ifndef IMPARO_TIMELINE
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -241,8 +244,9 @@ static inline cudaError_t timeline_note(const void*) { return cudaSuccess; }
 
 extern "C" int imparo_pdl_enabled();
 
+// early: the kernel may be scheduled before the one ahead of it in the stream has completed (its own wait orders what it reads)
 template <typename... KArgs, typename... Args>
-static inline cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+static inline cudaError_t launch_as(bool early, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
     {
         cudaError_t e = timeline_note(reinterpret_cast<const void*>(kernel));
         if (e != cudaSuccess) return e;
@@ -256,8 +260,17 @@ static inline cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = imparo_pdl_enabled() ? 1 : 0;
+    cfg.numAttrs = early ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
+template <typename... KArgs, typename... Args>
+static inline cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+    return launch_as(imparo_pdl_enabled() != 0, kernel, grid, block, smem, stream, args...);
+}
+// Starts only when all that is ahead of it in the stream is complete and visible, and whatever comes behind it starts later still.
+template <typename... KArgs, typename... Args>
+static inline cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+    return launch_as(false, kernel, grid, block, smem, stream, args...);
 }
 
 #define IMPARO_CHECK_LAUNCH() do { cudaError_t e__ = cudaGetLastError(); if (e__ != cudaSuccess) return (int)e__; } while (0)

@@ -7,10 +7,13 @@
 // of the counts before it, a token's slot is page * page_size + place in the page (64-bit: rows of a large arena pass 32 bits in
 // bytes long before, but slots are multiplied by a row's width by whoever uses them).
 //
-// One launch: a CTA owns some items and sums the counts and the pages taken over all items before them by itself; for the item
-// counts of a step (hundreds) that is one or two loads per thread, less than a second launch or a wait between CTAs costs.  On a B200
-// 2.9 us for 8 decode rows of 2,048 positions, 6.4 for 256 items of 32,768 (3.7 MB), 12.4 for 500 portions of 200 tokens, where every CTA
-// looks at the 13 blocks of each item before its own.
+// One launch makes it: a CTA owns some items and sums the counts and the pages taken over all items before them by itself; for the item
+// counts of a step (hundreds) that is one or two loads per thread, less than a launch before it or a wait between CTAs costs.
+//
+// A second, empty launch completes it: the engine's kernels read the description before they wait for the kernels ahead of them
+// (common.cuh), so nothing may start before it is there.  Both on a B200: 3.7 us for 8 decode rows of 2,048 positions, 7.0 for 256 items
+// of 32,768 (3.7 MB), 10.8 for 500 portions of 200 tokens, where every CTA looks at the 13 blocks of each item before its own.  The
+// empty launch adds 0.8 us to the first.
 #include "common.cuh"
 
 namespace imparo {
@@ -74,7 +77,7 @@ __device__ __forceinline__ long long warp_sum64(long long v) {
 __global__ void __launch_bounds__(THREADS)
 step_tables_kernel(const Args a) {
     __shared__ long long part[2][THREADS / 32];
-    pdl_trigger();
+    timeline_begin();                                          // (lets nothing start early: the launch behind it waits for all of it)
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int r0 = blockIdx.x * a.items_per_cta, r1 = min(a.n_items, r0 + a.items_per_cta);
@@ -157,6 +160,13 @@ step_tables_kernel(const Args a) {
     }
 }
 
+// Does nothing.  Every kernel of the engine reads the description of the step before it waits for the kernels ahead of it, so none may
+// start before the description is complete: this one is launched without that freedom, and they come behind it.
+__global__ void step_tables_complete_kernel() {
+    pdl_trigger();
+    pdl_wait();
+}
+
 }  // namespace st
 }  // namespace imparo
 
@@ -177,5 +187,6 @@ extern "C" int imparo_step_tables(const int* lengths, const int* counts, const i
     a.items_per_cta = (n_items + 1183) / 1184;                 // up to eight CTAs per SM
     const int ctas = (n_items + a.items_per_cta - 1) / a.items_per_cta;
     cudaError_t e = launch(st::step_tables_kernel, dim3(ctas), dim3(st::THREADS), 0, stream, a);
+    if (e == cudaSuccess) e = launch_after(st::step_tables_complete_kernel, dim3(1), dim3(32), 0, stream);
     return e == cudaSuccess ? 0 : (int)e;
 }

@@ -1646,6 +1646,7 @@ def step_tables(lengths, counts, free_pages, held, page_size, n_pages, table, po
                                              _ptr(parent), _ptr(shared), n, int(page_size), int(n_pages), at_table, width,
                                              positions.data_ptr(), item_of_token.data_ptr(), tokens, row_start.data_ptr(),
                                              slots.data_ptr(), taken.data_ptr(), status.data_ptr(), _stream()), "step_tables")
+    COUNTS["own"] += 1          # (the tables, and the launch that holds back what reads them)
 
 
 class SharedPrefixPlan(NamedTuple):

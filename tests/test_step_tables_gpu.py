@@ -185,6 +185,78 @@ def test_captured_and_replayed():
         assert np.array_equal(got.cpu().numpy(), np.asarray(want))
 
 
+@pytest.mark.parametrize("between", [False, True])
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_kernels_right_behind_read_the_new_tables(dtype, graph, between):
+    """The cache writer and the attention, launched behind the tables with nothing in between (or one more kernel of the chain): the
+    arrays hold another step's description before, as valid as the new one."""
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(1)
+    nh, nkv, hd, page, items, width, n_pages = 8, 2, 64, 16, 64, 40, 64 * 40
+    i32 = lambda v: torch.tensor(np.asarray(v, dtype=np.int32), device=DEV)
+    steps = []
+    for seed in (0, 1):
+        rng = np.random.default_rng(seed)
+        lengths, counts = rng.integers(0, 600, items), np.ones(items, dtype=np.int64)
+        pages = rng.permutation(n_pages)
+        held = np.full((items, width), -1)
+        at = 0
+        for r in range(items):
+            n = -(-int(lengths[r]) // page)
+            held[r, :n] = pages[at:at + n]
+            at += n
+        free = pages[at:at + items]
+        made = plain(lengths, counts, free, held, page, width, items)
+        steps.append(([i32(x) for x in (lengths, counts, free, held)], i32(made[0]), i32(made[1])))
+    item_of, row_start, slots, taken = i32(np.zeros(items)), i32(np.zeros(items + 1)), torch.zeros(items, dtype=torch.int64, device=DEV), i32([0])
+    table, positions = i32(np.zeros((items, width))), i32(np.zeros(items))
+    status = ops.new_status(DEV)
+    draw = lambda *shape: torch.randn(*shape, device=DEV, generator=gen).to(dtype)
+    qkv, first_k, first_v = draw(items, (nh + 2 * nkv) * hd), draw(n_pages, page, nkv * hd), draw(n_pages, page, nkv * hd)
+    inv_freq = 10000.0 ** (-torch.arange(hd // 2, device=DEV, dtype=torch.float32) / (hd // 2))
+    q, out, k, v = torch.empty(items, nh * hd, dtype=dtype, device=DEV), torch.empty(items, nh * hd, dtype=dtype, device=DEV), first_k.clone(), first_v.clone()
+    chunk, n_splits = ops.split_plan(items, nkv, width * page)
+    acc, ml = torch.empty(items * nh * n_splits * hd, device=DEV), torch.empty(items * nh * n_splits * 2, device=DEV)
+    some, weight, normed = torch.randn(4, 64, device=DEV, generator=gen), torch.ones(64, device=DEV), torch.empty(4, 64, device=DEV)
+
+    def reads(table, positions, item_of):
+        ops.qk_norm_rope_store(qkv, positions, item_of, None, None, inv_freq, hd, 1e-6, q, k, v, table, page, n_pages, nh, nkv, hd, status)
+        assert ops.paged_attention_split(q, k, v, positions, item_of, table, page, n_pages, None, hd ** -0.5, out, acc, ml, chunk, n_splits, nh,
+                                         nkv, hd, status)
+
+    def step(which):
+        ops.step_tables(*steps[which][0], page, n_pages, table, positions, item_of, row_start, slots, taken, status)
+        if between:
+            ops.rmsnorm(some, weight, 1e-6, normed)
+        reads(table, positions, item_of)
+
+    def whole(run):
+        k.copy_(first_k)
+        v.copy_(first_v)
+        torch.cuda.synchronize()
+        run()
+        torch.cuda.synchronize()
+        ops.read_status(status)
+        return q.clone(), out.clone(), k.clone(), v.clone()
+
+    order = i32(np.arange(items))
+    want = [whole(lambda: reads(steps[w][1], steps[w][2], order)) for w in (0, 1)]
+    assert not torch.equal(want[0][1], want[1][1])
+    graphs = []
+    for w in (0, 1):
+        step(w)
+        torch.cuda.synchronize()
+        if graph:
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1]):
+                step(w)
+    for n in range(12):
+        w = n % 2
+        for got, expected in zip(whole(graphs[w].replay if graph else lambda: step(w)), want[w]):
+            assert torch.equal(got, expected)
+
+
 def test_refusals():
     i32 = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=DEV)
     names = ("lengths", "counts", "free_pages", "held", "page_size", "n_pages", "table", "positions", "item_of_token", "row_start", "slots",
