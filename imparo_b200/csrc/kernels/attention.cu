@@ -19,7 +19,8 @@ constexpr int WARPS = 4;
 
 // What does not depend on the previous kernel is done before the wait on it: the token's
 // position, the norm weights, the rotation's sines and cosines and the cache row (the batch
-// description comes from the host before the step).  After the wait: one load of the head's
+// description is complete before the step's first kernel).  A token without a position (-1: a row of no request) has queries, but no
+// keys and values to keep: nothing is written to the cache for it, and nothing reported.  After the wait: one load of the head's
 // values, the norm, the rotation, the store.
 // FEW: at most eight partials (or none): straight-line loads, all of a head's values in flight together
 // PER: elements of a head per lane (head size up to 32 * PER), so that a head of 64 does not pay
@@ -71,7 +72,7 @@ qk_norm_rope_store_kernel(const T* __restrict__ qkv, const int* __restrict__ pos
         const int kvh = is_k ? hh - nh : hh - nh - nkv;
         const int blk = pos / page_size;
         int page = -1;
-        if (blk < max_blocks) page = table[(size_t)item_of_token[t] * max_blocks + blk];
+        if (pos >= 0 && blk < max_blocks) page = table[(size_t)item_of_token[t] * max_blocks + blk];
         if (page < 0 || page >= n_pages) {
             bad_page = page;                                 // reported after the wait
         } else {
@@ -81,7 +82,7 @@ qk_norm_rope_store_kernel(const T* __restrict__ qkv, const int* __restrict__ pos
     }
     pdl_wait();
     if (dst == nullptr) {
-        if (lane == 0) report(status, IMPARO_ST_PAGE_RANGE, 2, t, bad_page);
+        if (lane == 0 && pos >= 0) report(status, IMPARO_ST_PAGE_RANGE, 2, t, bad_page);
         return;
     }
 
@@ -181,7 +182,7 @@ qk_norm_rope_rows_kernel(const T* __restrict__ qkv, const int* __restrict__ posi
     int page = 0;
     if (nkv > 0) {
         const int blk = pos / page_size;
-        page = blk < max_blocks ? table[(size_t)item_of_token[t] * max_blocks + blk] : -1;
+        page = pos >= 0 && blk < max_blocks ? table[(size_t)item_of_token[t] * max_blocks + blk] : -1;
         if (page >= 0 && page < n_pages) cache_row = (size_t)page * page_size + (pos % page_size);
     }
     pdl_wait();
@@ -203,7 +204,7 @@ qk_norm_rope_rows_kernel(const T* __restrict__ qkv, const int* __restrict__ posi
             dst = q_out + (size_t)t * nh * hd + (size_t)hh * hd;
         } else {
             if (page < 0 || page >= n_pages) {
-                if (lane == 0) report(status, IMPARO_ST_PAGE_RANGE, 2, t, page);
+                if (lane == 0 && pos >= 0) report(status, IMPARO_ST_PAGE_RANGE, 2, t, page);
                 return;
             }
             const int kvh = is_k ? hh - nh : hh - nh - nkv;
@@ -282,11 +283,11 @@ qk_norm_rope_rows_vec_kernel(const __nv_bfloat16* __restrict__ qkv, const int* _
     int page = 0;
     if (nkv > 0) {
         const int blk = pos / page_size;
-        page = blk < max_blocks ? table[(size_t)item_of_token[t] * max_blocks + blk] : -1;
+        page = pos >= 0 && blk < max_blocks ? table[(size_t)item_of_token[t] * max_blocks + blk] : -1;
         if (page >= 0 && page < n_pages) cache_row = (size_t)page * page_size + (pos % page_size);
     }
     pdl_wait();
-    if (nkv > 0 && (page < 0 || page >= n_pages) && threadIdx.x == 0)
+    if (nkv > 0 && pos >= 0 && (page < 0 || page >= n_pages) && threadIdx.x == 0)
         report(status, IMPARO_ST_PAGE_RANGE, 2, t, page);     // the token's keys and values are skipped below, its queries written
     const __nv_bfloat16* src = qkv + (size_t)t * total * HD + V * lane;
     const bool upper = lane >= 16;
@@ -371,7 +372,7 @@ qk_norm_rope_token_warp_kernel(const __nv_bfloat16* __restrict__ qkv, const int*
     size_t cache_row = 0;
     if (nkv > 0) {
         const int blk = pos / page_size;
-        page = blk < max_blocks ? table[(size_t)item_of_token[t] * max_blocks + blk] : -1;
+        page = pos >= 0 && blk < max_blocks ? table[(size_t)item_of_token[t] * max_blocks + blk] : -1;
         if (page >= 0 && page < n_pages) cache_row = (size_t)page * page_size + (pos % page_size);
     }
     float wq[8], wk[8], sn[8], cs[8];
@@ -403,7 +404,7 @@ qk_norm_rope_token_warp_kernel(const __nv_bfloat16* __restrict__ qkv, const int*
         }
     }
     pdl_wait();
-    if (nkv > 0 && (page < 0 || page >= n_pages) && lane == 0)
+    if (nkv > 0 && pos >= 0 && (page < 0 || page >= n_pages) && lane == 0)
         report(status, IMPARO_ST_PAGE_RANGE, 2, t, page);     // the token's keys and values are skipped below, its queries written
     const __nv_bfloat16* src = qkv + (size_t)t * total * HD + 8 * sub;
     const bool upper = sub >= LPH / 2;

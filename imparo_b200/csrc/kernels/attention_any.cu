@@ -61,7 +61,7 @@ qkv_rotate_store_kernel(const T* __restrict__ qkv, const int* __restrict__ posit
         src = qkv + (size_t)t * in_width + (size_t)nh * hd + (is_k ? (size_t)kvh * hd : (size_t)nkv * hd + (size_t)kvh * vd);
         const int blk = pos / page_size;
         int page = -1;
-        if (blk < max_blocks) page = table[(size_t)item_of_token[t] * max_blocks + blk];
+        if (pos >= 0 && blk < max_blocks) page = table[(size_t)item_of_token[t] * max_blocks + blk];
         if (page < 0 || page >= n_pages) {
             bad_page = page;
         } else {
@@ -71,7 +71,7 @@ qkv_rotate_store_kernel(const T* __restrict__ qkv, const int* __restrict__ posit
     }
     pdl_wait();
     if (dst == nullptr) {
-        if (lane == 0) report(status, IMPARO_ST_PAGE_RANGE, 41, t, bad_page);
+        if (lane == 0 && pos >= 0) report(status, IMPARO_ST_PAGE_RANGE, 41, t, bad_page);
         return;
     }
     const int half = n_rot >> 1;
@@ -126,12 +126,12 @@ qkv_rotate_store_token_kernel(const T* __restrict__ qkv, const int* __restrict__
     int page = 0;
     if (nkv > 0) {
         const int blk = pos / page_size;
-        page = blk < max_blocks ? table[(size_t)item_of_token[t] * max_blocks + blk] : -1;
+        page = pos >= 0 && blk < max_blocks ? table[(size_t)item_of_token[t] * max_blocks + blk] : -1;
         if (page >= 0 && page < n_pages) cache_row = (size_t)page * page_size + (pos % page_size);
     }
     __syncthreads();
     pdl_wait();
-    if (nkv > 0 && (page < 0 || page >= n_pages) && threadIdx.x == 0)
+    if (nkv > 0 && pos >= 0 && (page < 0 || page >= n_pages) && threadIdx.x == 0)
         report(status, IMPARO_ST_PAGE_RANGE, 41, t, page);           // the token's keys and values are skipped, its queries written
     const int total = nh + 2 * nkv;
     const T* row = qkv + (size_t)t * in_width;
@@ -193,7 +193,7 @@ qkv_prepare_store_kernel(const float* __restrict__ qkv, size_t in_width, const f
     } else {
         const int blk = pos / page_size;
         int page = -1;
-        if (blk < max_blocks) page = table[(size_t)item_of_token[t] * max_blocks + blk];
+        if (pos >= 0 && blk < max_blocks) page = table[(size_t)item_of_token[t] * max_blocks + blk];
         if (page < 0 || page >= n_pages) {
             bad_page = page;
         } else {
@@ -203,7 +203,7 @@ qkv_prepare_store_kernel(const float* __restrict__ qkv, size_t in_width, const f
     }
     pdl_wait();
     if (dst == nullptr) {
-        if (lane == 0) report(status, IMPARO_ST_PAGE_RANGE, 43, t, bad_page);
+        if (lane == 0 && pos >= 0) report(status, IMPARO_ST_PAGE_RANGE, 43, t, bad_page);
         return;
     }
     const float* src = qkv + (size_t)t * in_width + col;
@@ -276,12 +276,12 @@ qkv_prepare_store_token_kernel(const float* __restrict__ qkv, size_t in_width, c
     const int half = inv_freq ? (n_rot >> 1) : 0;
     for (int i = threadIdx.x; i < half; i += blockDim.x) sincosf((float)pos * inv_freq[i], &sn_s[i], &cs_s[i]);
     const int blk = pos / page_size;
-    const int page = blk < max_blocks ? table[(size_t)item_of_token[t] * max_blocks + blk] : -1;
+    const int page = pos >= 0 && blk < max_blocks ? table[(size_t)item_of_token[t] * max_blocks + blk] : -1;
     const bool mapped = page >= 0 && page < n_pages;
     const size_t cache_row = mapped ? (size_t)page * page_size + (pos % page_size) : 0;
     __syncthreads();
     pdl_wait();
-    if (!mapped && threadIdx.x == 0 && blockIdx.y == 0) report(status, IMPARO_ST_PAGE_RANGE, 43, t, page);   // its keys and values are skipped
+    if (!mapped && pos >= 0 && threadIdx.x == 0 && blockIdx.y == 0) report(status, IMPARO_ST_PAGE_RANGE, 43, t, page);   // its keys and values are skipped
     const float* row = qkv + (size_t)t * in_width;
     T* kd = k_cache + cache_row * ((size_t)nkv * hd);
     T* vd_row = v_cache + cache_row * ((size_t)nkv * vd);
@@ -341,13 +341,13 @@ qkv_norm_rotate_store_kernel(const T* __restrict__ qkv, size_t in_width, const i
     bool mapped = true;
     if (nkv > 0) {
         const int blk = pos / page_size;
-        page = blk < max_blocks ? table[(size_t)item_of_token[t] * max_blocks + blk] : -1;
+        page = pos >= 0 && blk < max_blocks ? table[(size_t)item_of_token[t] * max_blocks + blk] : -1;
         mapped = page >= 0 && page < n_pages;
         if (mapped) cache_row = (size_t)page * page_size + (pos % page_size);
     }
     __syncthreads();
     pdl_wait();
-    if (!mapped && threadIdx.x == 0 && h_end > nh) report(status, IMPARO_ST_PAGE_RANGE, 44, t, page);    // its keys and values are skipped
+    if (!mapped && pos >= 0 && threadIdx.x == 0 && h_end > nh) report(status, IMPARO_ST_PAGE_RANGE, 44, t, page);    // its keys and values are skipped
     const T* row = qkv + (size_t)t * in_width;
     float* hv = head[warp];
     for (int hh = h_first + warp; hh < h_end; hh += ANY_WARPS) {
@@ -416,7 +416,7 @@ qkv_norm_rotate_store_vec_kernel(const __nv_bfloat16* __restrict__ qkv, size_t i
     const int half = inv_freq ? (n_rot >> 1) : 0, hl = half / 8;         // hl: lanes between an element's and its partner's
     for (int i = threadIdx.x; i < half; i += blockDim.x) sincosf((float)pos * inv_freq[i], &sn_s[i], &cs_s[i]);
     const int blk = pos / page_size;
-    const int page = blk < max_blocks ? table[(size_t)item_of_token[t] * max_blocks + blk] : -1;
+    const int page = pos >= 0 && blk < max_blocks ? table[(size_t)item_of_token[t] * max_blocks + blk] : -1;
     const bool mapped = page >= 0 && page < n_pages;
     const size_t cache_row = mapped ? (size_t)page * page_size + (pos % page_size) : 0;
     float qw[8], kw[8], cs[8], sn[8];
@@ -435,7 +435,7 @@ qkv_norm_rotate_store_vec_kernel(const __nv_bfloat16* __restrict__ qkv, size_t i
         }
     }
     pdl_wait();
-    if (!mapped && threadIdx.x == 0 && blockIdx.y == 0) report(status, IMPARO_ST_PAGE_RANGE, 45, t, page);      // its keys and values are skipped
+    if (!mapped && pos >= 0 && threadIdx.x == 0 && blockIdx.y == 0) report(status, IMPARO_ST_PAGE_RANGE, 45, t, page);      // its keys and values are skipped
     const __nv_bfloat16* row = qkv + (size_t)t * in_width;
     if (mapped) {                                               // the values, as they are
         const uint4* src = reinterpret_cast<const uint4*>(row + (size_t)(nh + nkv) * hd);

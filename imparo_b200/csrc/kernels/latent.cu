@@ -34,14 +34,14 @@ latent_norm_store_kernel(const float* __restrict__ proj, size_t stride, int q_of
     const int t = blockIdx.x;
     const bool is_q = blockIdx.y == 0;
     T* dst = nullptr;
-    int bad_page = 0;
+    int bad_page = 0, pos = 0;
     if (is_q) {
         dst = q_out + (size_t)t * q_rank;
     } else {
-        const int pos = positions[t];
+        pos = positions[t];
         const int blk = pos / page_size;
         int page = -1;
-        if (blk < max_blocks) page = table[(size_t)item_of_token[t] * max_blocks + blk];
+        if (pos >= 0 && blk < max_blocks) page = table[(size_t)item_of_token[t] * max_blocks + blk];
         if (page < 0 || page >= n_pages) bad_page = page;
         else dst = cache + ((size_t)page * page_size + (pos % page_size)) * c_rank;
     }
@@ -53,7 +53,7 @@ latent_norm_store_kernel(const float* __restrict__ proj, size_t stride, int q_of
     for (int i = threadIdx.x; i < n; i += blockDim.x) ss += src[i] * src[i];
     ss = block_sum(ss, scratch);
     if (dst == nullptr) {
-        if (threadIdx.x == 0) report(status, IMPARO_ST_PAGE_RANGE, 74, t, bad_page);
+        if (threadIdx.x == 0 && pos >= 0) report(status, IMPARO_ST_PAGE_RANGE, 74, t, bad_page);
         return;
     }
     const float scale = 1.0f / sqrtf(ss / (float)n + eps);
@@ -99,7 +99,7 @@ latent_rot_store_kernel(const float* __restrict__ proj, size_t stride, int heads
     const bool is_row = (int)blockIdx.y == q_blocks;
     const int blk = pos / page_size;
     int page = -1;
-    if (is_row && blk < max_blocks) page = table[(size_t)item_of_token[t] * max_blocks + blk];
+    if (is_row && pos >= 0 && blk < max_blocks) page = table[(size_t)item_of_token[t] * max_blocks + blk];
     const int half = n_rot / 2, tail = row_w - rank;
     const float fpos = (float)pos;
     for (int j = threadIdx.x; j < half; j += blockDim.x) {
@@ -152,7 +152,7 @@ latent_rot_store_kernel(const float* __restrict__ proj, size_t stride, int heads
     for (int i = threadIdx.x; i < rank; i += blockDim.x) ss += c[i] * c[i];
     ss = block_sum(ss, scratch);
     if (page < 0 || page >= n_pages) {
-        if (threadIdx.x == 0) report(status, IMPARO_ST_PAGE_RANGE, 75, t, page);
+        if (threadIdx.x == 0 && pos >= 0) report(status, IMPARO_ST_PAGE_RANGE, 75, t, page);
         return;
     }
     T* dst = cache + ((size_t)page * page_size + (pos % page_size)) * row_w;

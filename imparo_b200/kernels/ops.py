@@ -1130,7 +1130,8 @@ def qk_norm_rope_store(qkv, positions, item_of_token, q_w, k_w, inv_freq, n_rot,
                        k_cache, v_cache, table, page_size, n_pages, nh, nkv, hd, status) -> None:
     """qkv [T, (nh+2*nkv)*hd] (a tensor or a PartialProduct) -> q_out [T, nh*hd] normed and rotated;
     k (normed, rotated) and v written into their pages.  nkv == 0: q only (a layer that reads
-    another's cache).  q_w / k_w None: no per-head norm on that side (rotation only)."""
+    another's cache).  q_w / k_w None: no per-head norm on that side (rotation only).  A row of position -1 (no request's) writes
+    nothing to the cache; so it is with the other operators that write there."""
     src, parts, part_stride = _parts_of(qkv)
     _cuda(src, positions, item_of_token, q_w, k_w, inv_freq, q_out, k_cache, v_cache, table, status)
     T = q_out.shape[0]
@@ -1622,7 +1623,9 @@ def step_tables(lengths, counts, free_pages, held, page_size, n_pages, table, po
     not -1 are those that held[parent[r]] lists; the page in which the shared positions end, if they end inside one, is the item's
     own, and its shared part is for the caller to copy.
     row_start (int32 [items + 1]): each item's first token, and their number.  positions, item_of_token (int32) and slots (int64, page *
-    page_size + place) per token; entries behind the last token get position -1 (which attends to nothing), item 0 and slot -1.
+    page_size + place) per token; entries behind the last token get position -1, item 0 and slot -1.  A row of position -1 attends to
+    nothing, and what writes to the paged cache (qk_norm_rope_store and its like) skips it; operators that keep a state per item
+    (convolutions, recurrences) know no such rows and take those up to row_start[items] only.
     taken (int32 [1]): how many of the free pages are now in use.
 
     A free list that is too short, a table or token arrays that are too narrow, negative lengths, whole shared pages beyond lengths[r]
