@@ -217,7 +217,7 @@ shared_any_kernel(const Args a, const int aligned) {
     if (written) {
         const size_t at_part = ((size_t)t * a.nh + head) * n_splits + split;
         if (sub == 0) { a.part_ml[at_part * 2] = m; a.part_ml[at_part * 2 + 1] = l; }
-        if (l > 0.f) {
+        if (l != 0.f) {                                            // (a sum that is no number counts: the row has no result)
 #pragma unroll
             for (int i = 0; i < OUT; ++i)
                 if (4 * sub + 32 * i < hd) {
@@ -250,10 +250,8 @@ static int launch_any(const Args& a, cudaStream_t stream) {
 
 using namespace imparo;
 
-extern "C" int imparo_attention_split_combine(const float* part_acc, const float* part_ml, void* out, int dtype, int n_rows, int hd,
-                                              int n_splits, int sink, cudaStream_t stream);
-extern "C" int imparo_attention_split_combine_sinks(const float* part_acc, const float* part_ml, void* out, int dtype, int n_rows, int hd,
-                                                    int n_splits, const float* sink_values, int nh, cudaStream_t stream);
+extern "C" int imparo_attention_split_combine_any_sum(const float* part_acc, const float* part_ml, void* out, int dtype, int n_rows, int hd,
+                                                      int n_splits, const float* sink_values, int nh, cudaStream_t stream);
 
 extern "C" int imparo_attention_shared(const void* q, long long q_stride, const void* k_cache, const void* v_cache, int dtype,
                                        const int* positions, const int* item_of_token, const int* table, int n_items, int max_blocks,
@@ -281,7 +279,5 @@ extern "C" int imparo_attention_shared(const void* q, long long q_stride, const 
     if (rc == 0 && n_own == 1) return 0;                     // its second kernel has joined everything
     if (rc == -8) rc = dtype == IMPARO_DT_F32 ? sp::launch_any<float>(a, stream) : sp::launch_any<__nv_bfloat16>(a, stream);
     if (rc != 0) return rc;
-    if (sink_values)
-        return imparo_attention_split_combine_sinks(part_acc, part_ml, out, dtype, n_rows * nh, hd, n_shared + n_own, sink_values, nh, stream);
-    return imparo_attention_split_combine(part_acc, part_ml, out, dtype, n_rows * nh, hd, n_shared + n_own, 0, stream);
+    return imparo_attention_split_combine_any_sum(part_acc, part_ml, out, dtype, n_rows * nh, hd, n_shared + n_own, sink_values, nh, stream);
 }

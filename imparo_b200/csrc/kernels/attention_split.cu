@@ -238,8 +238,10 @@ attn_split_partial_kernel(const T* __restrict__ q, const T* __restrict__ k_cache
 // One block per (token, head): fold the splits in order.  Beyond 32 splits their (max, sum) pairs go
 // through shared memory and the first sixteen splits' accumulators are requested at the same
 // time, so the usual launch costs one round trip to memory.
+// ANY_SUM: a sum that is no number takes part, so that a row with a score that is none has no result either; otherwise its split is left
+// out, and the row comes out as if the split's keys were not there.
 constexpr int COMBINE_MAX_SPLITS = 2048;
-template <typename T>
+template <typename T, bool ANY_SUM = false>
 __global__ void attn_split_combine_kernel(const float* __restrict__ part_acc, const float* __restrict__ part_ml,
                                           T* __restrict__ out, int hd, int n_splits, int sink,
                                           const float* __restrict__ sink_values, int nh) {
@@ -248,6 +250,7 @@ __global__ void attn_split_combine_kernel(const float* __restrict__ part_acc, co
     __shared__ float m_all;
     pdl_trigger();
     pdl_wait();
+    auto holds = [](float sum) { return ANY_SUM ? sum != 0.f : sum > 0.f; };
     const size_t th = blockIdx.x;                         // token * nh + head
     const float sink_at = sink_values ? sink_values[th % nh] : 0.f;      // the extra term's score: 0, or a number per head
     const float* ml = part_ml + th * n_splits * 2;
@@ -262,11 +265,11 @@ __global__ void attn_split_combine_kernel(const float* __restrict__ part_acc, co
             float p[32];
 #pragma unroll
             for (int u = 0; u < 32; ++u) p[u] = u < n_splits && d < hd ? __ldcg(acc + (size_t)u * hd + d) : 0.f;
-            const unsigned live = __ballot_sync(0xffffffffu, v.y > 0.f);
-            float M = warp_max(v.y > 0.f ? v.x : -INFINITY);
+            const unsigned live = __ballot_sync(0xffffffffu, holds(v.y));
+            float M = warp_max(holds(v.y) ? v.x : -INFINITY);
             if (sink) M = fmaxf(M, sink_at);
-            const float f = v.y > 0.f ? expf(v.x - M) : 0.f;
-            float a = 0.f, L = sink ? expf(sink_at - M) : 0.f;
+            const float f = holds(v.y) ? expf(v.x - M) : 0.f;
+            float a = 0.f, L = sink && !(ANY_SUM && sink_at == -INFINITY) ? expf(sink_at - M) : 0.f;
 #pragma unroll
             for (int u = 0; u < 32; ++u) {
                 if (u % 8 == 0 && u >= n_splits) break;
@@ -276,7 +279,7 @@ __global__ void attn_split_combine_kernel(const float* __restrict__ part_acc, co
                     L += ls * fs;
                 }
             }
-            if (d < hd) out[th * hd + d] = from_f32<T>(L > 0.f ? a / L : 0.f);
+            if (d < hd) out[th * hd + d] = from_f32<T>(holds(L) ? a / L : 0.f);
         }
         return;
     }
@@ -291,17 +294,17 @@ __global__ void attn_split_combine_kernel(const float* __restrict__ part_acc, co
     __syncthreads();
     if (threadIdx.x < 32) {
         float M = -INFINITY;
-        for (int s = threadIdx.x; s < n_splits; s += 32) if (l_s[s] > 0.f) M = fmaxf(M, f_s[s]);
+        for (int s = threadIdx.x; s < n_splits; s += 32) if (holds(l_s[s])) M = fmaxf(M, f_s[s]);
         M = warp_max(M);
         if (sink) M = fmaxf(M, sink_at);                  // one more term (sum 1, no value) takes part in the fold
         if (threadIdx.x == 0) m_all = M;
     }
     __syncthreads();
     const float M = m_all;
-    for (int s = threadIdx.x; s < n_splits; s += blockDim.x) f_s[s] = l_s[s] > 0.f ? expf(f_s[s] - M) : 0.f;
+    for (int s = threadIdx.x; s < n_splits; s += blockDim.x) f_s[s] = holds(l_s[s]) ? expf(f_s[s] - M) : 0.f;
     __syncthreads();
     for (int d = d0; d < hd; d += blockDim.x) {
-        float a = 0.f, L = sink ? expf(sink_at - M) : 0.f;
+        float a = 0.f, L = sink && !(ANY_SUM && sink_at == -INFINITY) ? expf(sink_at - M) : 0.f;
         for (int s0 = 0; s0 < n_splits; s0 += 16) {
             if (s0 > 0 || d != d0) {
 #pragma unroll
@@ -309,13 +312,13 @@ __global__ void attn_split_combine_kernel(const float* __restrict__ part_acc, co
             }
 #pragma unroll
             for (int u = 0; u < 16; ++u) {
-                if (s0 + u < n_splits && l_s[s0 + u] > 0.f) {
+                if (s0 + u < n_splits && holds(l_s[s0 + u])) {
                     a += pa[u] * f_s[s0 + u];
                     L += l_s[s0 + u] * f_s[s0 + u];
                 }
             }
         }
-        out[th * hd + d] = from_f32<T>(L > 0.f ? a / L : 0.f);
+        out[th * hd + d] = from_f32<T>(holds(L) ? a / L : 0.f);
     }
 }
 
@@ -421,6 +424,24 @@ extern "C" int imparo_attention_split_combine_sinks(const float* part_acc, const
     else if (dtype == IMPARO_DT_BF16)
         launch(attn_split_combine_kernel<__nv_bfloat16>, dim3(n_rows), dim3(threads), 0, stream, part_acc, part_ml, (__nv_bfloat16*)out,
                hd, n_splits, 1, sink_values, nh);
+    else return -1;
+    IMPARO_CHECK_LAUNCH();
+    return 0;
+}
+
+// The combine for partial results whose sums may be no number: such a split takes part (a NaN row comes out as NaN).  sink_values: as
+// above, or null.
+extern "C" int imparo_attention_split_combine_any_sum(const float* part_acc, const float* part_ml, void* out, int dtype, int n_rows, int hd,
+                                                      int n_splits, const float* sink_values, int nh, cudaStream_t stream) {
+    if (n_rows <= 0) return 0;
+    if (n_splits < 1 || n_splits > COMBINE_MAX_SPLITS || nh < 1) return -2;
+    const int threads = hd >= 128 ? 128 : (hd >= 64 ? 64 : 32), sink = sink_values ? 1 : 0;
+    if (dtype == IMPARO_DT_F32)
+        launch(attn_split_combine_kernel<float, true>, dim3(n_rows), dim3(threads), 0, stream, part_acc, part_ml, (float*)out, hd, n_splits,
+               sink, sink_values, nh);
+    else if (dtype == IMPARO_DT_BF16)
+        launch(attn_split_combine_kernel<__nv_bfloat16, true>, dim3(n_rows), dim3(threads), 0, stream, part_acc, part_ml, (__nv_bfloat16*)out, hd,
+               n_splits, sink, sink_values, nh);
     else return -1;
     IMPARO_CHECK_LAUNCH();
     return 0;

@@ -342,6 +342,53 @@ class TestManyRows:
         assert torch.equal(got[3:], want[3:])
 
 
+@pytest.mark.parametrize("where", ["shared", "own"])
+@pytest.mark.parametrize("dtype,hd,rows,most_own", [(torch.float32, 64, 4, 40), (torch.float32, 64, 4, 2000), (torch.bfloat16, 96, 4, 40),
+                                                    (torch.bfloat16, 64, 4, 40), (torch.bfloat16, 64, 4, 2000), (torch.bfloat16, 64, 90, 40),
+                                                    (torch.bfloat16, 128, 4, 40), (torch.bfloat16, 128, 4, 2000), (torch.bfloat16, 128, 90, 40)])
+class TestNoNumbers:
+    """A score that is no number or infinite, in whichever stretch of whichever kernel: who sees it has no result, the others theirs."""
+
+    def setup(self, where, dtype, hd, rows, most_own):
+        b = Batch([(rows, 200)], 40, 4, 2, hd, dtype)
+        plan = ops.shared_prefix_plan(rows, 1, 4, 2, hd, dtype, 200, most_own)
+        pos = 77 if where == "shared" else 215                     # an own one is row 1's alone
+        place = b.k[b.table[1, pos // 16], pos % 16]
+        sees = torch.ones(rows, dtype=torch.bool, device=DEV) if where == "shared" else torch.arange(rows, device=DEV) == 1
+        return b, plan, place, sees
+
+    def test_a_key_that_is_no_number(self, where, dtype, hd, rows, most_own):
+        b, plan, place, sees = self.setup(where, dtype, hd, rows, most_own)
+        want = b.run(plan=plan).view(rows, 4, hd)
+        place[3] = float("nan")                                    # of the first kv head: query heads 0 and 1
+        got = b.run(plan=plan).view(rows, 4, hd)
+        assert got[sees, :2].isnan().all()
+        assert torch.equal(got[sees, 2:], want[sees, 2:]) and torch.equal(got[~sees], want[~sees])
+
+    def test_an_infinite_score(self, where, dtype, hd, rows, most_own):
+        """Above all others: none has a finite share.  Below all: a share of 0, as that of a very low score."""
+        b, plan, place, sees = self.setup(where, dtype, hd, rows, most_own)
+        q = b.q.view(rows, 4, hd)
+        q[:, 0, 0], q[:, 1, 0] = 1.0, -1.0
+        place[0] = 1e30
+        want = b.run(plan=plan).view(rows, 4, hd)
+        assert want.isfinite().all()
+        place[0] = float("inf")
+        got = b.run(plan=plan).view(rows, 4, hd)
+        assert got[sees, 0].isnan().all()
+        assert torch.equal(got[sees, 1:], want[sees, 1:]) and torch.equal(got[~sees], want[~sees])
+
+    def test_a_query_that_is_no_number(self, where, dtype, hd, rows, most_own):
+        b, plan, _, _ = self.setup(where, dtype, hd, rows, most_own)
+        sinks = torch.tensor([0.5, -1.0, 2.0, 0.0], device=DEV) if where == "own" else None
+        want = b.run(plan=plan, sinks=sinks).view(rows, 4, hd)
+        b.q[2, hd + 5] = float("nan")                              # row 2, head 1
+        got = b.run(plan=plan, sinks=sinks).view(rows, 4, hd)
+        assert got[2, 1].isnan().all()
+        want[2, 1] = got[2, 1] = 0
+        assert torch.equal(got, want)
+
+
 def test_no_rows():
     b = Batch([(2, 30)], 2, 4, 2, 64, torch.bfloat16)
     plan = ops.shared_prefix_plan(1, 1, 4, 2, 64, torch.bfloat16, 30, 2)
