@@ -151,7 +151,8 @@ def new_status(device) -> torch.Tensor:
 
 
 _STATUS_TEXT = {1: "token id out of the vocabulary", 2: "cache page out of range (unmapped block or bad table)",
-                3: "state slot out of range", 4: "a bounded device wait gave up (tensor-core product)"}
+                3: "state slot out of range", 4: "a bounded device wait gave up (tensor-core product)",
+                5: "a step's description does not fit (too few free pages, table or token arrays too small, bad lengths, counts or parents)"}
 
 
 def read_status(status: torch.Tensor) -> None:

@@ -59,3 +59,18 @@ def test_plan_refusals():
                  (1, 1, 4, 2, 64, torch.float32, -1, 1), (1, 1, 4, 2, 64, torch.float32, 1, -1)):
         with pytest.raises(ops.KernelError):
             ops.shared_prefix_plan(*args, sms=148)
+
+
+def test_every_status_code_has_a_text():
+    """The codes of csrc/kernels/common.cuh; what read_status says names the cause, not the code."""
+    import os
+    import re
+    header = os.path.join(os.path.dirname(ops.__file__), "..", "csrc", "kernels", "common.cuh")
+    with open(header) as f:
+        codes = {name: int(code) for name, code in re.findall(r"#define IMPARO_ST_(\w+) (\d+)", f.read())}
+    assert codes["STEP_SIZE"] == 5
+    for code in codes.values():
+        status = torch.tensor([code, 63, 2, -1], dtype=torch.int32)
+        with pytest.raises(ops.KernelError, match=r"device check failed: [a-z][^0-9]{8,}\(kernel 63, index 2, value -1\)"):
+            ops.read_status(status)
+        assert not status.any()

@@ -185,6 +185,18 @@ def test_captured_and_replayed():
         assert np.array_equal(got.cpu().numpy(), np.asarray(want))
 
 
+@pytest.mark.parametrize("change,code,where", [
+    (dict(free=[5, 6]), 5, 63), (dict(width=3), 5, 61), (dict(n_tokens=33), 5, 65), (dict(lengths=[20, -5, 0]), 5, 60),
+    (dict(counts=[30, -3, 2]), 5, 60), (dict(parent=[-1, 3, -1], shared=[0, 16, 0]), 5, 62), (dict(parent=[-1, 0, -1], shared=[0, 16, 0]), 5, 66),
+    (dict(held=[[0, 10], [2, -1], [-1, -1]]), 2, 64), (dict(free=[5, 600, 7, 8, 9]), 2, 63)])
+def test_what_does_not_fit_is_named(change, code, where):
+    args = dict(lengths=[20, 5, 0], counts=[30, 3, 2], free=[5, 6, 7, 8, 9], held=[[0, 1], [2, -1], [-1, -1]], page=16, n_pages=10, width=4, n_tokens=35)
+    _, status = device_call(**{**args, **change})
+    assert status.tolist()[:2] == [code, where]
+    with pytest.raises(ops.KernelError, match="step's description" if code == 5 else "cache page out of range"):
+        ops.read_status(status)
+
+
 @pytest.mark.parametrize("between", [False, True])
 @pytest.mark.parametrize("graph", [False, True])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
