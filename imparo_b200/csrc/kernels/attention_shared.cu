@@ -1,6 +1,6 @@
 // Attention of single-token rows whose first positions are the same pages of the cache: continuations of one prompt, or questions
 // behind one document.  The rows are cut into groups; the positions 0 .. shared - 1 of a group's rows are read by the block table of
-// its first row, once for all of its rows, the rest of each row by its own table.
+// its first row that has a position, once for all of its rows, the rest of each row by its own table.
 //
 //   o_t = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q_t . k_j),  lo_t <= j <= pos_t        (lo_t = 0, or pos_t + 1 - window)
 //
@@ -52,24 +52,22 @@ shared_any_kernel(const Args a, const int aligned) {
     int unit = blockIdx.z;
     const int head0 = unit % head_tiles * ROWS;
     unit /= head_tiles;
-    int row0, n_tok, group, tab_of;                                // the tokens of this tile, the row whose table gives the pages
+    int row0, n_tok, group;                                        // the tokens of this tile
     if (is_own) {
         if (unit >= a.n_rows) return;
         row0 = unit;
         n_tok = 1;
-        tab_of = row0;
         group = group_of_warp(a, row0);
     } else {
         group = 0;
         n_tok = 0;
-        row0 = tab_of = 0;
+        row0 = 0;
         for (; group < a.n_groups; ++group) {
             int start, end;
             group_rows(a, group, start, end);
             const int tiles = (end - start + tokens_per - 1) / tokens_per;
             if (unit < tiles) {
                 row0 = start + unit * tokens_per;
-                tab_of = start;
                 n_tok = min(tokens_per, end - row0);
                 break;
             }
@@ -98,6 +96,7 @@ shared_any_kernel(const Args a, const int aligned) {
     const Own own = own_keys(a, a.positions[row0], span);
     const int total = is_own ? own.count : span.end - span.first;
     const int k0 = (int)min((long long)at * chunk, (long long)total), k1 = last ? total : (int)min((long long)k0 + chunk, (long long)total);
+    const int tab_of = is_own ? row0 : span.row;                   // the row whose table gives the pages
     const int* tab = k0 < k1 ? table_row(a, tab_of, 70) : nullptr;
 
     const size_t kvw = (size_t)a.nkv * hd;

@@ -62,22 +62,24 @@ __device__ __forceinline__ int first_seen(const Args& a, int pos) { return a.win
 
 // The keys [first, end) that the shared stretches take for a group: those of its shared positions that every row of it sees (rows
 // without a position, pos < 0, aside).  Each row takes the rest of what it sees, on both sides of them, with its own ones, so the
-// shared stretches need no mask by row and whatever a row does not see never meets its weights.  Every warp finds it by itself (no
-// barrier); the result is the same for every launch of the same arrays.
-struct Span { int first, end; };
+// shared stretches need no mask by row and whatever a row does not see never meets its weights.  The pages are those that the first row with a
+// position lists: one without may have ended and its pages be gone, and a group of nothing but such rows has no shared keys.  Every warp
+// finds all this by itself (no barrier); the result is the same for every launch of the same arrays.
+struct Span { int first, end, row; };
 __device__ __forceinline__ Span shared_span(const Args& a, int g) {
-    if (g < 0) return Span{0, 0};
+    if (g < 0) return Span{0, 0, 0};
     int start, end;
     group_rows(a, g, start, end);
-    int lo = 0, hi = max(0, a.shared[g]);
+    int lo = 0, hi = max(0, a.shared[g]), row = a.n_rows;
 #pragma unroll 4
     for (int t = start + (threadIdx.x & 31); t < end; t += 32) {
         const int pos = min(a.positions[t], a.most_pos);
-        if (pos >= 0) { lo = max(lo, first_seen(a, pos)); hi = min(hi, pos + 1); }
+        if (pos >= 0) { lo = max(lo, first_seen(a, pos)); hi = min(hi, pos + 1); row = min(row, t); }
     }
     lo = __reduce_max_sync(0xffffffffu, lo);
     hi = __reduce_min_sync(0xffffffffu, hi);
-    return lo < hi ? Span{lo, hi} : Span{0, 0};
+    row = __reduce_min_sync(0xffffffffu, row);
+    return row < a.n_rows && lo < hi ? Span{lo, hi, row} : Span{0, 0, 0};
 }
 // A row's own keys, counted through: the first `before` of them lie before the shared ones.  (A position far beyond the table is an
 // error that the first key without a block reports; without the bound the row would look up every one of up to 2^31 keys.)

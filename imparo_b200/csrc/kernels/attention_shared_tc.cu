@@ -209,7 +209,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         // Keys and values are fetched as their buffers come free, whichever first.  Where the copies' rows lie is looked up a
         // thousand copies at a time: a lookup per copy is a trip to memory that every step then waits for.
         int* where = reinterpret_cast<int*>(bars + 64);      // [PAGES] first cache row of copy c of the CTA's, at c % PAGES
-        const int* tab = table_row(a, start, 72);
+        const int* tab = table_row(a, span.row, 72);
         const int box = min(a.page_size, STEP), log_copies = box == 16 ? 2 : box == 32 ? 1 : 0, copies = 1 << log_copies;
         const int first_blk = span.first / a.page_size, last_blk = (span.end - 1) / a.page_size;
         int known = 0;
@@ -220,7 +220,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 const int key = first_step * STEP + c * box, blk = min(max(key / a.page_size, first_blk), last_blk);
                 int page = tab != nullptr && blk < a.max_blocks ? tab[blk] : -1;
                 if (page < 0 || page >= a.n_pages) {
-                    report(a.status, IMPARO_ST_PAGE_RANGE, 73, start, page);
+                    report(a.status, IMPARO_ST_PAGE_RANGE, 73, span.row, page);
                     page = 0;
                 }
                 where[c % C::PAGES] = page * a.page_size + key % a.page_size;

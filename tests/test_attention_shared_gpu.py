@@ -258,6 +258,27 @@ class TestRows:
                 ops.read_status(b.status)
             assert torch.equal(got[4:], want[4:])
 
+    def test_a_group_of_rows_without_a_position_looks_nothing_up(self, dtype, hd):
+        """All of its continuations have ended and their pages are gone, whatever its shared length still says."""
+        b = Batch([(4, 200), (3, 150), (2, 64)], 30, 4, 2, hd, dtype)
+        want = b.run()
+        b.positions[4:7] = -1
+        b.table[4:7] = -1
+        for shared in (150, 0x7fffffff):
+            b.shared[1] = shared
+            got = b.run()
+            assert not got[4:7].any() and torch.equal(got[:4], want[:4]) and torch.equal(got[7:], want[7:])
+
+    def test_the_first_continuations_of_a_group_have_ended(self, dtype, hd):
+        b = Batch([(1, 40), (40, 200), (2, 64)], 30, 4, 2, hd, dtype)
+        plan = ops.shared_prefix_plan(43, 3, 4, 2, hd, dtype, 200, 30)
+        b.positions[1:36] = -1
+        want = b.run(plan=plan)
+        b.table[1:36] = -1
+        b.items[1:36] = 0
+        got = b.run(plan=plan)
+        assert torch.equal(got, want) and not got[1:36].any() and got[36:41].any(dim=1).all()
+
     def test_captured_and_replayed(self, dtype, hd):
         b = Batch([(4, 300), (2, 64)], lambda r: 9 + r, 4, 2, hd, dtype)
         plan = ops.shared_prefix_plan(6, 2, 4, 2, hd, dtype, 300, 20)
