@@ -799,7 +799,7 @@ own_tc_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __rest
             }
             if (sinks) {
                 const float sink = sinks[head0 + h] * LOG2E, m_new = fmaxf(m, sink), corr = m == -INFINITY ? 0.f : ex2(m - m_new);
-                l = l * corr + ex2(sink - m_new);
+                l = l * corr + (sink == -INFINITY ? 0.f : ex2(sink - m_new));        // (minus infinity: no sink, for a row of nothing too)
 #pragma unroll
                 for (int e = 0; e < PER; ++e) acc[e] *= corr;
             }
@@ -1027,7 +1027,7 @@ own_ring_kernel(const Args a, __nv_bfloat16* __restrict__ out, const float* __re
     }
     if (sinks) {
         const float sink = sinks[head0 + g] * LOG2E, m_new = fmaxf(m, sink), corr = m == -INFINITY ? 0.f : ex2(m - m_new);
-        l = l * corr + ex2(sink - m_new);
+        l = l * corr + (sink == -INFINITY ? 0.f : ex2(sink - m_new));        // (minus infinity: no sink, for a row of nothing too)
 #pragma unroll
         for (int i = 0; i < NB * 8; ++i) { o[i][0] *= corr; o[i][1] *= corr; }
     }

@@ -177,6 +177,19 @@ class TestRows:
         b = Batch([(4, 300)], lambda r: 1 + 3 * r, 8, 2, hd, dtype)
         b.check(sinks=torch.tensor([-50.0, -2.0, 0.0, 1.0, 3.0, 8.0, 30.0, 80.0], device=DEV))
 
+    @pytest.mark.parametrize("rows", [6, 90])
+    @pytest.mark.parametrize("most_own", [20, 2000])
+    def test_sinks_of_minus_infinity_are_none(self, dtype, hd, rows, most_own):
+        """exp(-inf) adds nothing: as without a sink, and zeros for a row that sees nothing."""
+        b = Batch([(rows, 100)], 20, 4, 2, hd, dtype)
+        b.positions[1] = -1
+        plan = ops.shared_prefix_plan(rows, 1, 4, 2, hd, dtype, 100, most_own)
+        want = b.run(plan=plan)
+        some = torch.tensor([float("-inf"), 0.5, float("-inf"), -1.0], device=DEV)
+        got = b.run(plan=plan, sinks=some).view(rows, 4, hd)
+        assert not got[1].any() and torch.equal(got[:, ::2], want.view(rows, 4, hd)[:, ::2])
+        assert torch.equal(b.run(plan=plan, sinks=torch.full((4,), float("-inf"), device=DEV)), want)
+
     def test_rows_without_a_position_and_rows_that_end_inside_the_shared_part(self, dtype, hd):
         b = Batch([(6, 260), (2, 40)], 9, 8, 2, hd, dtype, extra=1)
         pos = b.positions.clone()
