@@ -257,7 +257,7 @@ sample_filtered_kernel(const Args a) {
                 f(v, Places{i, 1});
                 raw = next;
             }
-            if (whole < to) {                                      // the last ones, by the first lanes
+            if (from <= whole && whole < to) {                     // the last ones, by the first lanes (an empty part has none)
                 const float v[4] = {whole + lane < to ? load1(row + whole + lane) : -INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 f(v, Places{whole + lane, 32});
             }

@@ -89,6 +89,18 @@ def test_vocabulary_beyond_shared_memory():
           [0, 0, 0, 0, 0, 1e-3, 0])
 
 
+@pytest.mark.parametrize("vocab", [140000, 140001, 140002, 140003])
+def test_picks_among_the_last_entries_of_a_long_row(vocab):
+    """The row's end is no multiple of four, and parts of its last stretch are empty: each entry is weighed once."""
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((6, vocab)).astype(np.float32)
+    x[:, -9:] += 12.0
+    u = [1 - 2.0 ** -24, 0.999, 0.97, 0.9, 0.6, 0.3]
+    for k, p, m in (([0] * 6, [1.0] * 6, [0.0] * 6), ([0] * 6, [0.99] * 6, [0.0] * 6), ([100000] * 6, [1.0] * 6, [1e-9] * 6)):
+        got = check(torch.tensor(x, device=DEV), [1.0] * 6, u, k, p, m)
+        assert got[0][0] == vocab - 1 or p[0] < 1
+
+
 @pytest.mark.parametrize("vocab", [4096, 40000])
 def test_equal_logits_stay_by_index(vocab):
     logits = torch.zeros(9, vocab, device=DEV)
