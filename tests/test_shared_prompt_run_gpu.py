@@ -117,6 +117,121 @@ def test_several_continuations_of_two_prompts(dtype, graph):
     assert len(free) < 60 - 9                                      # pages were taken on the way
 
 
+@pytest.mark.parametrize("dtype,hd", [(torch.float32, 64), (torch.bfloat16, 64), (torch.bfloat16, 128)])
+def test_a_padded_step_is_captured_once(dtype, hd):
+    """Eight continuations of two prompts, of which others rest or have ended in every step: tables, cache rows and attention, with nothing
+    between them, in one graph for eight rows.  The rows behind the step's tokens change nothing; the others are as in a step of their number."""
+    nh, nkv, page, n_pages, width, rows = 8, 2, 16, 100, 12, 8
+    rng = np.random.default_rng(hd)
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(hd)
+    i32 = lambda x: torch.tensor(np.asarray(x, dtype=np.int32), device=DEV)
+    new = lambda n: i32(np.zeros(n))
+    prompts, of = [80, 32], [0, 0, 0, 0, 0, 1, 1, 1]
+    free = list(range(n_pages))                                    # (page 0 is the first prompt's first)
+    whole = [[free.pop(0) for _ in range(n // page)] for n in prompts]
+    held = np.full((rows, width), -1)
+    for r, g in enumerate(of):
+        held[r, :len(whole[g])] = whole[g]
+    lengths = np.array([prompts[g] for g in of])
+    draw = lambda *shape: torch.randn(*shape, device=DEV, generator=gen).to(dtype)
+    k = torch.cat([torch.full((1, page, nkv * hd), 5.0, device=DEV, dtype=dtype), draw(n_pages, page, nkv * hd)])        # a page before the arena
+    v = k.flip(0).contiguous()
+    k_plain, v_plain = k.clone(), v.clone()
+    inv_freq = 10000.0 ** (-torch.arange(hd // 2, device=DEV, dtype=torch.float32) / (hd // 2))
+    plan = ops.shared_prefix_plan(rows, 2, nh, nkv, hd, dtype, 80, 30)
+    acc, ml, status = torch.empty(plan.acc_floats, device=DEV), torch.empty(plan.ml_floats, device=DEV), ops.new_status(DEV)
+    qkv, q, out = draw(rows, (nh + 2 * nkv) * hd), torch.zeros(rows, nh * hd, dtype=dtype, device=DEV), torch.zeros(rows, nh * hd, dtype=dtype, device=DEV)
+
+    def reads(qkv, q, k, v, positions, items, table, group_start, shared, out):
+        ops.qk_norm_rope_store(qkv, positions, items, None, None, inv_freq, hd, 1e-6, q, k[1:], v[1:], table, page, n_pages, nh, nkv, hd, status)
+        ops.paged_attention_shared(q, k[1:], v[1:], positions, items, table, page, n_pages, group_start, shared, None, hd ** -0.5, out, acc, ml,
+                                   plan, nh, nkv, hd, status)
+
+    lens, counts, free_dev, held_dev, shared = i32(lengths), new(rows), new(rows), i32(held), i32(prompts)
+    table, positions, items, start, slots, taken = torch.empty_like(held_dev), new(rows), new(rows), new(rows + 1), torch.zeros(rows, dtype=torch.int64, device=DEV), new(1)
+    group_start = i32([0, 5, 8])
+
+    def step():
+        ops.step_tables(lens, counts, free_dev, held_dev, page, n_pages, table, positions, items, start, slots, taken, status)
+        reads(qkv, q, k, v, positions, items, table, group_start, shared, out)
+
+    def replay():
+        nonlocal graph
+        if graph is None:
+            step()                                                 # (kernels configure themselves at their first launch)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                step()
+        graph.replay()
+
+    graph = None
+    for n in range(8):
+        active = np.array([1] * 8 if n == 0 else [0] * 8 if n == 7 else rng.integers(0, 2, 8))
+        if n == 5:
+            active[:5] = 0                                         # the first group rests
+        for dst, src in ((lens, lengths), (counts, active), (free_dev, free[:rows]), (held_dev, held),
+                         (group_start, [0, active[:5].sum(), active.sum()])):
+            dst.copy_(i32(src))
+        qkv.copy_(draw(*qkv.shape))
+        replay()
+        ops.read_status(status)
+        t = int(active.sum())
+        who = np.flatnonzero(active)
+        for r in who:
+            if held[r, lengths[r] // page] < 0:
+                held[r, lengths[r] // page] = free.pop(0)
+        assert positions.tolist() == lengths[who].tolist() + [-1] * (rows - t)
+        if t:
+            q_plain, out_plain = torch.zeros(t, nh * hd, dtype=dtype, device=DEV), torch.zeros(t, nh * hd, dtype=dtype, device=DEV)
+            reads(qkv[:t], q_plain, k_plain, v_plain, i32(lengths[who]), i32(who), i32(held), group_start, shared, out_plain)
+            assert torch.equal(out[:t], out_plain) and out_plain.any()
+        assert not out[t:].any() and torch.equal(k, k_plain) and torch.equal(v, v_plain)
+        lengths[who] += 1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_two_streams_at_once(dtype):
+    """Two programs' steps side by side on one device, each with buffers of its own: as one after the other."""
+    batches = [Batch([(20, 700), (3, 100)], lambda r: 1 + 5 * r, 8, 2, 64, dtype, seed=s) for s in (1, 2)]
+    rng = np.random.default_rng(1)
+    logits = [torch.tensor(rng.standard_normal((5, 30000)) * 2, dtype=torch.float32, device=DEV) for _ in range(2)]
+    ones, half = torch.ones(5, device=DEV), torch.full((5,), 0.5, device=DEV)
+    i32 = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=DEV)
+    plan = ops.shared_prefix_plan(23, 2, 8, 2, 64, dtype, 700, 120)
+    programs = []
+    for b, x in zip(batches, logits):
+        table, positions, items = torch.empty_like(b.table), i32(23), i32(23)
+        scratch = [torch.empty(plan.acc_floats, device=DEV), torch.empty(plan.ml_floats, device=DEV)]
+        made = [table, positions, items, i32(24), torch.zeros(23, dtype=torch.int64, device=DEV), i32(1)]
+        lens, counts, free, out, ids = b.positions.clone(), i32(23) + 1, i32(1), torch.empty_like(b.q), i32(5)
+
+        def step(b=b, x=x, made=made, scratch=scratch, lens=lens, counts=counts, free=free, out=out, ids=ids):
+            ops.step_tables(lens, counts, free, b.table, b.page, b.n_pages, *made, b.status)
+            ops.paged_attention_shared(b.q, b.k, b.v, made[1], made[2], made[0], b.page, b.n_pages, b.group_start, b.shared, None, b.scale, out,
+                                       *scratch, plan, 8, 2, 64, b.status)
+            ops.sample_filtered(x, ones, half, ids, top_p=half)
+        programs.append((step, out, ids, b))
+    want = []
+    for step, out, ids, _ in programs:
+        step()
+        torch.cuda.synchronize()
+        want.append((out.clone(), ids.clone()))
+        out.zero_()
+        ids.zero_()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for stream, (step, *_rest) in zip(streams, programs):
+            with torch.cuda.stream(stream):
+                step()
+    torch.cuda.synchronize()
+    for (_, out, ids, b), (w_out, w_ids) in zip(programs, want):
+        ops.read_status(b.status)
+        assert torch.equal(out, w_out) and torch.equal(ids, w_ids)
+
+
 def test_sampler_rows_with_and_without_filters():
     """A row without a filter is picked as it always was, whatever its neighbours ask for."""
     rng = np.random.default_rng(4)
