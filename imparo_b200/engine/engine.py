@@ -38,7 +38,7 @@ def checked_filters(n: int, top_ks: Sequence[int], top_ps: Sequence[float], min_
     for name, values in (("top_k", top_ks), ("top_p", top_ps), ("min_p", min_ps)):
         if len(values) != n:
             raise ValueError(f"{name}: {len(values)} values for {n} prompts")
-    if any(int(k) != k or k < 0 for k in top_ks):
+    if not all(float(k).is_integer() and k >= 0 for k in top_ks):
         raise ValueError("top_k must be a whole number, 0 (all tokens) or more")
     if not all(0 < p <= 1 for p in top_ps):
         raise ValueError("top_p must be above 0 and at most 1 (all tokens)")
