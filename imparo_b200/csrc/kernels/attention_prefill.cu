@@ -330,7 +330,7 @@ attn_decode_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16*
     float* wacc = wl + 32;                                             // [4][8][HD]
     pdl_trigger();
 
-    // the batch description (positions, block table) comes from the host before the step: it is
+    // the batch description (positions, block table) is complete before the step's first kernel: it is
     // read, and the chunk's table entries are pulled into the L1, before the wait on the previous kernel
     const int split = blockIdx.x, kvh = blockIdx.y, t = blockIdx.z;
     const int G = nh / nkv;

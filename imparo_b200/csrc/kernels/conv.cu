@@ -103,7 +103,7 @@ __device__ __forceinline__ void conv_portion_head(const ConvIn<T, MODE>& bcx, co
 }
 
 // The batch description (which request a token belongs to, where its portion starts, its state
-// slot) comes from the host before the step and the taps are weights: both are read before the
+// slot) is complete before the step's first kernel and the taps are weights: both are read before the
 // wait on the previous kernel, so that after it only activations and state remain to be fetched.
 template <typename T, int MODE>
 __global__ void gated_conv_kernel(const ConvIn<T, MODE> bcx, const float* __restrict__ w,

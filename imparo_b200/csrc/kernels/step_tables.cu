@@ -11,9 +11,9 @@
 // counts of a step (hundreds) that is one or two loads per thread, less than a launch before it or a wait between CTAs costs.
 //
 // A second, empty launch completes it: the engine's kernels read the description before they wait for the kernels ahead of them
-// (common.cuh), so nothing may start before it is there.  Both on a B200: 3.7 us for 8 decode rows of 2,048 positions, 7.0 for 256 items
-// of 32,768 (3.7 MB), 10.8 for 500 portions of 200 tokens, where every CTA looks at the 13 blocks of each item before its own.  The
-// empty launch adds 0.8 us to the first.
+// (common.cuh), so nothing may start before it is there.  Both on a B200: 4.0 us for 8 decode rows of 2,048 positions, 7.4 for 256 items
+// of 32,768 (3.7 MB), 11.1 for 500 portions of 200 tokens, where every CTA looks at the 13 blocks of each item before its own.  The
+// empty launch adds about 1 us to the first two.
 #include "common.cuh"
 
 namespace imparo {

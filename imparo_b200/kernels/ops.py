@@ -1710,7 +1710,8 @@ def paged_attention_shared(q, k_cache, v_cache, positions, item_of_token, table,
     q [rows, nh * hd] may be a slice of wider rows; out is dense.  float32 or bfloat16, head sizes that are multiples of 16 up to 256.
     window: None, or the number of last positions a row sees.  A row of position -1 sees nothing, needs no pages and gives zeros.  A row and head that
     sees a score of NaN or plus infinity gives NaN, whatever the plan; minus infinity is a weight of 0.
-    sink_values (float32 [nh]): one more term exp(value) in each head's denominator.
+    sink_values (float32 [nh]): one more term exp(value) in each head's denominator.  There is no cap on the scores: layers that cap them
+    go through paged_attention_split.
     plan: shared_prefix_plan() for these rows; part_acc and part_ml: the caller's scratch of plan.acc_floats and plan.ml_floats float32
     entries, not to be shared by calls that may run at the same time."""
     if not q.is_cuda or q.dim() != 2 or q.stride(1) != 1:
