@@ -133,3 +133,30 @@ def test_a_page_that_is_missing_is_still_reported():
     ops.qk_norm_rope_store(rand(1, 1, 256), zero, zero, None, None, inv(64), 64, 1e-6, q, k, v, table, PAGE, PAGES, 2, 1, 64, status)
     with pytest.raises(ops.KernelError):
         ops.read_status(status)
+
+
+@pytest.mark.parametrize("window", [None, 20])
+@pytest.mark.parametrize("which,dtype", [("any head", F32), ("any head", BF16), ("split", F32), ("split", BF16), ("general", F32), ("general", BF16),
+                                         ("shared heads", BF16), ("sigmoid", BF16)])
+def test_attention_of_rows_without_a_position_is_zero(which, dtype, window):
+    nh, nkv, hd, rows = 4, 2, 64, 9
+
+    def call(T, positions, items, table, caches, status):
+        q, out = rand(1, 40, nh * hd, dtype=dtype)[:T].contiguous(), torch.full((T, nh * hd), 3.0, dtype=dtype, device=DEV)
+        caches = [rand(5 + i, PAGES, PAGE, nkv * hd, dtype=dtype) for i in range(2)]
+        chunk, n_splits = ops.split_plan(rows, nkv, table.shape[1] * PAGE)
+        acc, ml = torch.empty(T * nh * n_splits * hd, device=DEV), torch.empty(T * nh * n_splits * 2, device=DEV)
+        head = (q, *caches, positions, items, table, PAGE, PAGES, window)
+        if which == "any head":
+            ops.paged_attention(*head, 0.125, out, nh, nkv, hd, status)
+        elif which == "split":
+            assert ops.paged_attention_split(*head, 0.125, out, acc, ml, chunk, n_splits, nh, nkv, hd, status)
+        elif which == "general":
+            ops.attention_any(*head, 0.125, True, out, nh, nkv, hd, hd, status)
+        elif which == "shared heads":
+            assert ops.paged_attention_split_shared(*head, 0.125, out, acc, ml, chunk, n_splits, nh, nkv, hd, status)
+        else:
+            assert ops.attention_sigmoid_split(*head, None, 0.125, torch.zeros(nh, device=DEV), out, acc, ml, chunk, n_splits, nh, nkv, hd, hd, status)
+        assert not out[rows:].any() and out[:rows].any(dim=1).all()
+        return [out]
+    run(call, rows, dtype, [8])
