@@ -62,9 +62,9 @@ __device__ __forceinline__ int first_seen(const Args& a, int pos) { return a.win
 
 // The keys [first, end) that the shared stretches take for a group: those of its shared positions that every row of it sees (rows
 // without a position, pos < 0, aside).  Each row takes the rest of what it sees, on both sides of them, with its own ones, so the
-// shared stretches need no mask by row and whatever a row does not see never meets its weights.  The pages are those that the first row with a
-// position lists: one without may have ended and its pages be gone, and a group of nothing but such rows has no shared keys.  Every warp
-// finds all this by itself (no barrier); the result is the same for every launch of the same arrays.
+// shared stretches need no mask by row and whatever a row does not see never meets its weights.  The pages are those that the first row
+// with a position lists: one without may have ended and its pages be gone, and a group of nothing but such rows has no shared keys.
+// Every warp finds all this by itself (no barrier); the result is the same for every launch of the same arrays.
 struct Span { int first, end, row; };
 __device__ __forceinline__ Span shared_span(const Args& a, int g) {
     if (g < 0) return Span{0, 0, 0};

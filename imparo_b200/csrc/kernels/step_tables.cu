@@ -160,7 +160,7 @@ step_tables_kernel(const Args a) {
     }
 }
 
-// Does nothing.  Every kernel of the engine reads the description of the step before it waits for the kernels ahead of it, so none may
+// Does nothing.  The engine's kernels read the description of the step before they wait for the kernels ahead of them, so none may
 // start before the description is complete: this one is launched without that freedom, and they come behind it.
 __global__ void step_tables_complete_kernel() {
     pdl_trigger();

@@ -1704,12 +1704,12 @@ def paged_attention_shared(q, k_cache, v_cache, positions, item_of_token, table,
                            sink_values: Optional[torch.Tensor] = None) -> None:
     """paged_attention for rows that share their first positions: the rows group_start[g] .. group_start[g + 1] - 1 (int32 [groups + 1])
     have the same keys and values at the positions 0 .. shared_len[g] - 1 (int32 [groups]), which are read once for all of them, by
-    the table row of the group's first row that has a position; the rest of each row's positions, up to its own, by its own table row, which lists all
-    of its pages as in paged_attention.  A group of one row and rows behind the last group are rows that share nothing.
+    the table row of the group's first row that has a position; the rest of each row's positions, up to its own, by its own table row,
+    which lists all of its pages as in paged_attention.  A group of one row and rows behind the last group are rows that share nothing.
 
     q [rows, nh * hd] may be a slice of wider rows; out is dense.  float32 or bfloat16, head sizes that are multiples of 16 up to 256.
-    window: None, or the number of last positions a row sees.  A row of position -1 sees nothing, needs no pages and gives zeros.  A row and head that
-    sees a score of NaN or plus infinity gives NaN, whatever the plan; minus infinity is a weight of 0.
+    window: None, or the number of last positions a row sees.  A row of position -1 sees nothing, needs no pages and gives zeros.  A row
+    and head that sees a score of NaN or plus infinity gives NaN, whatever the plan; minus infinity is a weight of 0.
     sink_values (float32 [nh]): one more term exp(value) in each head's denominator.  There is no cap on the scores: layers that cap them
     go through paged_attention_split.
     plan: shared_prefix_plan() for these rows; part_acc and part_ml: the caller's scratch of plan.acc_floats and plan.ml_floats float32
